@@ -1,6 +1,6 @@
 """Build testtimeideas_amd/_ttt_torch.so, the torch binding of the C entry
-points (ttt_torch.cpp), against the in-tree libttt_attn.so (found next
-to the module through an $ORIGIN run path).  The object goes to _build/ext.
+points (ttt_torch.cpp, ttt_ops_torch.cpp), against the in-tree libttt_attn.so (found next
+to the module through an $ORIGIN run path).  The objects go to _build/ext.
 Run after the library is built (``make -C testtimeideas_amd/csrc``)."""
 import os
 import subprocess
@@ -11,6 +11,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
 ROOT = os.path.dirname(PKG)
 NAME = "_ttt_torch"
+SOURCES = ("ttt_torch", "ttt_ops_torch")
 
 
 def build(verbose: bool = False) -> str:
@@ -18,20 +19,25 @@ def build(verbose: bool = False) -> str:
 
     out_dir = os.path.join(ROOT, "_build", "ext")
     os.makedirs(out_dir, exist_ok=True)
-    obj = os.path.join(out_dir, "ttt_torch.o")
+    objs = [os.path.join(out_dir, name + ".o") for name in SOURCES]
     dst = os.path.join(PKG, NAME + ".so")
     inc = [f"-I{p}" for p in cpp_extension.include_paths()] + [f"-I{sysconfig.get_paths()['include']}",
                                                               "-I/opt/rocm/include"]
     cflags = ["-O2", "-fPIC", "-std=c++17", f"-DTORCH_EXTENSION_NAME={NAME}", "-DTORCH_API_INCLUDE_EXTENSION_H",
               "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1"]
-    compile_cmd = ["c++", *cflags, *inc, "-c", os.path.join(HERE, "ttt_torch.cpp"), "-o", obj]
+    compile_cmds = [["c++", *cflags, *inc, "-c", os.path.join(HERE, name + ".cpp"), "-o", obj]
+                    for name, obj in zip(SOURCES, objs)]
     libs = [f"-L{p}" for p in cpp_extension.library_paths()]
-    link_cmd = ["c++", "-shared", obj, "-o", dst + ".tmp", f"-L{PKG}", "-lttt_attn", "-Wl,-rpath,$ORIGIN", *libs,
+    link_cmd = ["c++", "-shared", *objs, "-o", dst + ".tmp", f"-L{PKG}", "-lttt_attn", "-Wl,-rpath,$ORIGIN", *libs,
                 "-lc10_hip", "-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
-    for cmd in (compile_cmd, link_cmd):
-        if verbose:
+    if verbose:
+        for cmd in (*compile_cmds, link_cmd):
             print(" ".join(cmd), flush=True)
-        subprocess.run(cmd, check=True)
+    jobs = [subprocess.Popen(cmd) for cmd in compile_cmds]  # side by side
+    for job, cmd in zip(jobs, compile_cmds):
+        if job.wait():
+            raise subprocess.CalledProcessError(job.returncode, cmd)
+    subprocess.run(link_cmd, check=True)
     os.replace(dst + ".tmp", dst)
     return dst
 

@@ -20,6 +20,7 @@
 
 #include "../../include/ttt_attn.h"
 #include "ttt_launch.h"
+#include "ttt_ops.h"
 
 namespace {
 
@@ -32,6 +33,18 @@ int fail(int code, const char* fmt, ...) {
   va_end(ap);
   return code;
 }
+
+}  // namespace
+
+int ttt::ops_fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+namespace {
 
 // The split of a streamed loop into chunks is chosen by simulating how the
 // hardware would run the launch: workgroups go to the XCDs round-robin in

@@ -431,7 +431,10 @@ std::vector<at::Tensor> bwd_graph(const at::Tensor& q, const at::Tensor& k, cons
 
 }  // namespace
 
+void bind_ops(py::module_& m);  // ttt_ops_torch.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  bind_ops(m);
   m.doc() = "torch binding of the forward, backward and double backward of libttt_attn.so";
   m.def("fwd", &fwd, "forward: (O, LSE, P or None)");
   m.def("bwd", &bwd, "first backward: (dQ, dK, dV, D)");
