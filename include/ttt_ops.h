@@ -114,17 +114,19 @@ int ttt_lce_fwd(const ttt_lce_problem* problem, const ttt_rows* x, const ttt_row
                 const float* row_weight, float* loss, float* row_stats, void* workspace, int64_t workspace_bytes,
                 void* stream);
 
-/* grad_loss: fp32, of loss's shape.  dx or dw may be NULL. */
+/* grad_loss: fp32, of loss's shape.  dx or dw may be NULL.  dx32 ([rows, cols]
+ * contiguous, or NULL): dx before its rounding, for ttt_lce_gg. */
 int ttt_lce_bwd(const ttt_lce_problem* problem, const ttt_rows* x, const ttt_rows* w, const int64_t* target,
                 const float* row_weight, const float* row_stats, const float* grad_loss, const ttt_rows* dx,
-                const ttt_rows* dw, void* workspace, int64_t workspace_bytes, void* stream);
+                const ttt_rows* dw, float* dx32, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* a, b: cotangents of dx and dw; either may be NULL (zero), not both.  Any of
- * gx, gw and ggrad_loss (of loss's shape) may be NULL. */
+ * gx, gw and ggrad_loss (of loss's shape) may be NULL.  dx32: what ttt_lce_bwd
+ * wrote, or NULL (h is then summed from tiles, a third more work). */
 int ttt_lce_gg(const ttt_lce_problem* problem, const ttt_rows* x, const ttt_rows* w, const int64_t* target,
-               const float* row_weight, const float* row_stats, const float* grad_loss, const ttt_rows* a,
-               const ttt_rows* b, const ttt_rows* gx, const ttt_rows* gw, float* ggrad_loss, void* workspace,
-               int64_t workspace_bytes, void* stream);
+               const float* row_weight, const float* row_stats, const float* grad_loss, const float* dx32,
+               const ttt_rows* a, const ttt_rows* b, const ttt_rows* gx, const ttt_rows* gw, float* ggrad_loss,
+               void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

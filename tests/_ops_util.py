@@ -129,6 +129,10 @@ def lce_ref(x, w, t, wt, up, inv, dtype, a=None, b=None):
         4 * F32 * (a.abs() @ w.abs().t() + x.abs() @ b.abs().t()) / d ** 0.5
     hs = (p * uu).sum(1, keepdim=True)
     dh = (p * (du + rp * uu.abs())).sum(1, keepdim=True) + acc(v) * (p * uu.abs()).sum(1, keepdim=True)
+    # h may come from dX and G B, sums over the rounded G: u of each term of A . (|G| |W|) / c
+    ra = (a.abs() * (eg @ w.abs() + acc(v) * (g.abs() @ w.abs()))).sum(1, keepdim=True)
+    rb = (x.abs() * (eg @ b.abs() + acc(v) * (g.abs() @ b.abs()))).sum(1, keepdim=True)
+    dh = dh + torch.where(c != 0, (ra + rb) / c.abs().clamp_min(1e-300), 0.0)
     h = c * p * (uu - hs)
     eh = c.abs() * p * (rp * (uu - hs).abs() + du + dh) + 2 * F32 * h.abs() + (u if two else 4 * F32) * h.abs()
     if dtype == torch.float16:

@@ -29,14 +29,15 @@ def _weights(s):
     return torch.where(s["t"] == -100, 0.0, wt).double()
 
 
-def _run(s, names=("a", "b"), reduction="mean", up=None):
+def _run(s, names=("a", "b"), reduction="mean", up=None, up_grad=True):
+    """up_grad: the incoming gradient asks for its own (another way to form h)."""
     x, w = s["x"].cuda().requires_grad_(), s["w"].cuda().requires_grad_()
     mask = None if s["mask"] is None else s["mask"].cuda()
     loss = linear_cross_entropy(x, w, s["t"].cuda(), mask, reduction=reduction)
-    up = (torch.ones_like(loss) if up is None else up.cuda()).requires_grad_()
+    up = (torch.ones_like(loss) if up is None else up.cuda()).requires_grad_(up_grad)
     first = torch.autograd.grad(loss, (x, w), up, create_graph=True)
     pairs = [(f, s[k].cuda()) for f, k in zip(first, ("a", "b")) if k in names]
-    second = torch.autograd.grad([p[0] for p in pairs], (x, w, up), [p[1] for p in pairs])
+    second = torch.autograd.grad([p[0] for p in pairs], (x, w, up) if up_grad else (x, w), [p[1] for p in pairs])
     loss_name, up_name = ("rows", "gup") if reduction == "none" else ("loss", "gloss")
     return dict(zip((loss_name, "dx", "dw", "gx", "gw", up_name), (loss, *first, *second)))
 
@@ -60,6 +61,7 @@ SIZES = [(1, 1, 1), (1, 512, 4096), (1, 64, 1000), (2, 3, 5), (7, 24, 33), (65, 
 def test_values_and_both_gradients(n, d, v, dtype):
     s = _inputs(n, d, v, dtype, seed=n + d + v)
     _check(s, _run(s))
+    _check(s, _run(s, up_grad=False))
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
@@ -100,8 +102,9 @@ def test_second_gradient_of_one_operand():
 def test_pieces_of_the_vocabulary(dtype):
     """Enough rows times vocabulary that the gradients run in several pieces,
     the last one short."""
-    s = _inputs(2050, 40, 9001 if dtype == torch.float32 else 20011, dtype, seed=5, ignored=True)
+    s = _inputs(8200, 24, 33001, dtype, seed=5, ignored=True)
     _check(s, _run(s))
+    _check(s, _run(s, up_grad=False))
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
@@ -115,14 +118,15 @@ def test_many_pieces_of_the_statistics(dtype):
 def test_rows_that_do_not_count_may_hold_anything(dtype):
     s = _inputs(140, 64, 200, dtype, seed=7, masked=True, ignored=True)
     dead = _weights(s) == 0
-    clean = _run(s)
+    clean = [_run(s, up_grad=u) for u in (True, False)]
     s["x"][dead] = float("nan")
     s["x"][dead.nonzero()[0]] = float("inf")
     s["a"][dead] = float("nan")
-    got = _run(s)
-    for k in got:
-        assert torch.equal(got[k], clean[k]), k
-    assert not got["dx"][dead.cuda()].any() and not got["gx"][dead.cuda()].any()
+    for u in (True, False):
+        got = _run(s, up_grad=u)
+        for k in got:
+            assert torch.equal(got[k], clean[1 - u][k]), k
+        assert not got["dx"][dead.cuda()].any() and not got["gx"][dead.cuda()].any()
 
 
 @pytest.mark.parametrize("how", ["ignored", "masked"])
@@ -220,8 +224,17 @@ def test_python_refusals_on_the_gpu():
 
 def test_repeats_bitwise():
     s = _inputs(700, 120, 900, torch.bfloat16, seed=14, masked=True)
-    one, two = _run(s), _run(s)
-    assert all(torch.equal(one[k], two[k]) for k in one)
+    for u in (True, False):
+        one, two = _run(s, up_grad=u), _run(s, up_grad=u)
+        assert all(torch.equal(one[k], two[k]) for k in one)
+
+
+def test_no_upstream_gradient():
+    """Upstream 0: gradients 0, but the gradient of the upstream itself is not."""
+    s = _inputs(50, 64, 80, torch.bfloat16, seed=20)
+    got = _run(s, up=torch.tensor(0.0))
+    _check(s, {k: got[k] for k in ("loss", "gloss")}, up=0.0)
+    assert not any(got[k].any() for k in ("dx", "dw", "gx", "gw")) and got["gloss"] != 0
 
 
 def test_third_derivative_raises():

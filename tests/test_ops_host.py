@@ -105,9 +105,10 @@ def _lce(name, ws=P, wsn=1 << 50, x=None, w=None, **kw):
     if name == "fwd":
         return lib.ttt_lce_fwd(pr, x, w, t, None, _vp(P), _vp(P), _vp(ws), _i(wsn), None)
     if name == "bwd":
-        return lib.ttt_lce_bwd(pr, x, w, t, None, _vp(P), _vp(P), _rows(s), _rows(s), _vp(ws), _i(wsn), None)
-    return lib.ttt_lce_gg(pr, x, w, t, None, _vp(P), _vp(P), None, None, _rows(s), _rows(s), None, _vp(ws), _i(wsn),
-                          None)
+        return lib.ttt_lce_bwd(pr, x, w, t, None, _vp(P), _vp(P), _rows(s), _rows(s), None, _vp(ws), _i(wsn),
+                               None)
+    return lib.ttt_lce_gg(pr, x, w, t, None, _vp(P), _vp(P), None, None, None, _rows(s), _rows(s), None, _vp(ws),
+                          _i(wsn), None)
 
 
 def test_lce_refusals():
@@ -131,10 +132,10 @@ def test_lce_refusals():
 
 
 def test_lce_workspace_does_not_grow_with_the_logits():
-    """Four times the vocabulary: far less than four times the workspace."""
+    """Past a piece's size, the workspace is that of a piece."""
     size = lambda v, e: _c().ttt_lce_workspace_size(ctypes.byref(Lce(1, 2, 8192, 512, v, -100)), e)  # noqa: E731
-    assert size(1 << 18, 1) <= 1.1 * size(1 << 16, 1) and size(1 << 18, 2) <= 1.3 * size(1 << 16, 2)
-    assert size(1 << 18, 1) < 8192 * (1 << 18) * 2 / 8
+    assert all(size(1 << 22, e) <= 1.1 * size(1 << 17, e) for e in (0, 1, 2))
+    assert size(1 << 22, 1) < 8192 * (1 << 22) * 2 / 64
     assert size(0, 1) == -1 and size(64, 3) == -1
 
 

@@ -1,149 +1,221 @@
-// ttt_gemm.h — the tile product that the linear cross entropy's kernels are
+// ttt_gemm.h — the tile products that the linear cross entropy's kernels are
 // made of: a BM x BN tile of  sum_k Mop[m][k] Nop[n][k]  over a list of
 // segments, on the 16-bit matrix cores of gfx950.
 //
-// Both operands are row-major with k contiguous.  A segment is a pair of
-// operands and their common k; the sum runs over all segments in order.  That
-// one form covers
-//   - a plain product (one segment);
-//   - a contraction over two stacked ranges, [H | G] [W ; B] (two segments);
-//   - fp32 operands, each held as three bf16 parts whose sum is the value: six
-//     segments, the part products above 2^-24 of the whole, smallest first.
+// An operand is a row-major matrix in either order: its rows are m (or n) and
+// k is contiguous, or its rows are k and m is contiguous ("turned").  So no
+// product needs a transposed copy, and one order of G serves both dX = G W and
+// dW = G^T X.  A segment is a pair of operands and their common k; the sum
+// runs over all segments in order, which covers a contraction over two stacked
+// ranges, [H | G] [W ; B], without stacking them.
 //
 // MFMA 16x16x32: a lane (c = lane % 16, g = lane / 16) holds the results of
 // four consecutive m (4g ..) of one n (c).  So the M operand is chosen to be
 // the one whose index is contiguous in the output, and a token's sums over the
 // vocabulary stay in one lane plus two lane swaps.
 //
-// A step is 64 k: both tiles go straight from global memory to LDS (1 KB per
-// wave instruction: eight rows of 128 bytes, 16-byte chunks permuted by the
-// row's low three bits against bank conflicts), two buffers, the next step's
-// loads issued before this step's products.  Rows past an operand's end and
-// chunks past its k read as zeros through the buffer's range check.
+// TileProduct (16-bit types): a step is 64 k.  Both tiles go straight from
+// global memory to LDS (1 KB per wave instruction, 16-byte chunks permuted
+// against bank conflicts), two buffers, the next step's loads issued before
+// this step's products.  Turned tiles are read with ds_read_b64_tr_b16.  What
+// lies past an operand's end reads as zeros through the buffer's range check.
+//
+// SplitProduct (fp32): a value is the sum of three bf16 parts, exactly
+// (split_pair), and a product the sum of the six part products above 2^-22 of
+// it, smallest first, in fp32: six times the matrix work of bf16, where the
+// fp32 instruction takes sixteen.  A step is 32 k: values go to registers one
+// step ahead, are split once and stored as three tiles of parts; either order
+// of an operand ends up the same there.
 #pragma once
 
 #include "ttt_common.h"
 
 namespace ttt {
 
-constexpr int kStepK = 64;  // k of one step: 128 bytes of a row
-
 struct Seg {
-  const void *m, *n;  // first rows of the operands
+  const void *m, *n;  // first elements of the operands
   int64_t ldm, ldn;   // row strides in elements
-  int k;              // a multiple of 8
+  int k;
 };
 
-constexpr int kMaxSegs = 12;
+constexpr int kMaxSegs = 2;
 
 struct SegList {
   Seg s[kMaxSegs];
-  int n;      // segments
-  int steps;  // 64-k steps of all of them
+  int n;
 };
 
-// One operand's share of a step's loads: this lane's byte offsets.
-template <int ROWS, int NW>
-struct RowLoader {
-  static constexpr int kInstr = ROWS * 128 / 1024;
-  static constexpr int kPerWave = kInstr / NW;
-  static_assert(kPerWave * NW == kInstr, "tile shape");
-  uint32_t off[kPerWave];
+// Steps of STEP k in a list.
+template <int STEP>
+__host__ __device__ __forceinline__ int list_steps(const SegList& l) {
+  int t = 0;
+  for (int i = 0; i < l.n; ++i) t += (l.s[i].k + STEP - 1) / STEP;
+  return t;
+}
 
-  // rows_valid rows of stride ld elements
-  __device__ __forceinline__ void rows(int rows_valid, int64_t ld, int wave) {
-    const int lane = threadIdx.x & 63, r8 = lane >> 3;
-    const uint32_t ldb = (uint32_t)(ld * 2);
-#pragma unroll
-    for (int q = 0; q < kPerWave; ++q) {
-      const int r = 8 * (wave + NW * q) + r8;
-      off[q] = r < rows_valid ? (uint32_t)r * ldb + 16u * (uint32_t)((lane & 7) ^ r8) : kBufRange;
-    }
-  }
-  // base: the tile's first row at this step's k; past: this lane's chunk lies past the segment's k
-  __device__ __forceinline__ void issue(char* lds, const char* base, bool past, int wave) const {
-#if defined(__HIP_DEVICE_COMPILE__)
-    const __amdgpu_buffer_rsrc_t r =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), (short)0, (int)kBufRange, kBufWord3);
-#pragma unroll
-    for (int q = 0; q < kPerWave; ++q)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void_t*)(lds + 1024 * (wave + NW * q)), 16,
-                                               past ? kBufPast : (int)off[q], 0, 0, 0);
-#endif
-  }
-};
-
-template <typename T, int BM_, int BN_, int WM_, int WN_>
-struct TileProduct {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NW = WM * WN;
+// What the two products share: the waves' places in the tile, and the walk
+// over the segments.  Derived classes have enter() and the loads of a step.
+template <int BM_, int BN_, int WM_, int WN_, int STEP_>
+struct TileBase {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NW = WM * WN, kStep = STEP_;
   static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
-  typedef typename Elem<T>::frag frag;
-
-  // The four step buffers, in distinct arrays: the compiler waits for pending
-  // direct loads before an LDS read that may alias their destination.
-  struct Lds {
-    char *m0, *m1, *n0, *n1;
-  };
 
   int wave, wm, wn;
   int m0, n0, mrows, nrows;  // the tile's corner and the rows it has of each operand
-  RowLoader<BM, NW> lm;
-  RowLoader<BN, NW> ln;
+  int seg, k0;               // position in the segment list
 
-  __device__ __forceinline__ TileProduct(int m0_, int n0_, int M, int N) : m0(m0_), n0(n0_) {
+  __device__ __forceinline__ TileBase(int m0_, int n0_, int M, int N) : m0(m0_), n0(n0_) {
     wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     wm = wave % WM;
     wn = wave / WM;
     mrows = M - m0;
     nrows = N - n0;
   }
-
-  // Position in the segment list.
-  int seg, k0;
-  const char *bm, *bn;
-
-  __device__ __forceinline__ void enter(const SegList& l) {
-    const Seg& s = l.s[seg];
-    bm = (const char*)s.m + ((int64_t)m0 * s.ldm + k0) * 2;
-    bn = (const char*)s.n + ((int64_t)n0 * s.ldn + k0) * 2;
-    lm.rows(mrows, s.ldm, wave);
-    ln.rows(nrows, s.ldn, wave);
-  }
   __device__ __forceinline__ void seek(const SegList& l, int step) {
     seg = 0;
-    for (int n; seg + 1 < l.n && step >= (n = (l.s[seg].k + kStepK - 1) / kStepK); ++seg) step -= n;
-    k0 = step * kStepK;
-    enter(l);
+    for (int n; seg + 1 < l.n && step >= (n = (l.s[seg].k + kStep - 1) / kStep); ++seg) step -= n;
+    k0 = step * kStep;
+  }
+  __device__ __forceinline__ static void zero(f32x4 (&acc)[MI][NI]) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  // First m (of four) of acc[i][*] and the n of acc[*][j] in this lane.
+  __device__ __forceinline__ int m_of(int i) const { return m0 + (wm * MI + i) * 16 + 4 * ((threadIdx.x & 63) >> 4); }
+  __device__ __forceinline__ int n_of(int j) const { return n0 + (wn * NI + j) * 16 + (threadIdx.x & 15); }
+};
+
+// One 16-bit operand's share of a step's loads: this lane's byte offsets.
+//   plain:  LDS [R rows][64 k], chunk ^ (row & 7)
+//   turned: LDS [64 k][R], chunk ^ swz(k): the sixteen rows of a transposing
+//           read (k = 0-3, 8-11, 16-19, 24-27 past its first) are spread over
+//           eight 32-byte places
+template <int R, int NW, bool TURNED>
+struct Loader {
+  static constexpr int kInstr = R * 128 / 1024, kPerWave = kInstr / NW;
+  static_assert(kPerWave * NW == kInstr, "tile shape");
+  static constexpr int kRowBytes = TURNED ? R * 2 : 128, kChunks = kRowBytes / 16;
+  uint32_t off[kPerWave];
+  int64_t step;  // bytes from a step's first element to the next one's
+
+  static __device__ __forceinline__ int swz(int k) {
+    return ((k & 1) << 1) | (((k >> 1) & 1) << 2) | (((k >> 3) & 1) << 3);
+  }
+  static __device__ __forceinline__ int row_of(int q, int wave) {
+    return (1024 * (wave + NW * q) + 16 * (int)(threadIdx.x & 63)) / kRowBytes;
+  }
+  static __device__ __forceinline__ int chunk_of(int row) {
+    const int slot = (int)(threadIdx.x & 63) % kChunks;
+    return slot ^ (TURNED ? swz(row) : row & 7);
+  }
+  // valid: rows (turned: columns) of the tile that exist
+  __device__ __forceinline__ void enter(int valid, int64_t ld, int wave) {
+    step = TURNED ? 128 * ld : 128;
+#pragma unroll
+    for (int q = 0; q < kPerWave; ++q) {
+      const int r = row_of(q, wave), ch = chunk_of(r);
+      const bool in = TURNED ? 8 * ch < valid : r < valid;
+      off[q] = in ? (uint32_t)r * (uint32_t)(ld * 2) + 16u * (uint32_t)ch : kBufRange;
+    }
+  }
+  // base: the tile's first element at this step; left: k from here to the segment's end
+  __device__ __forceinline__ void issue(char* lds, const char* base, int left, int wave) const {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const __amdgpu_buffer_rsrc_t r =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), (short)0, (int)kBufRange, kBufWord3);
+    if (left >= 64) {
+#pragma unroll
+      for (int q = 0; q < kPerWave; ++q)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void_t*)(lds + 1024 * (wave + NW * q)), 16, (int)off[q], 0, 0,
+                                                 0);
+    } else {
+#pragma unroll
+      for (int q = 0; q < kPerWave; ++q) {
+        const int row = row_of(q, wave);
+        const bool in = TURNED ? row < left : 8 * chunk_of(row) < left;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void_t*)(lds + 1024 * (wave + NW * q)), 16,
+                                                 in ? (int)off[q] : kBufPast, 0, 0, 0);
+      }
+    }
+#endif
+  }
+};
+
+template <typename T, int BM_, int BN_, int WM_, int WN_, bool MT, bool NT>
+struct TileProduct : TileBase<BM_, BN_, WM_, WN_, 64> {
+  typedef TileBase<BM_, BN_, WM_, WN_, 64> B;
+  using B::BM;
+  using B::BN;
+  using B::MI;
+  using B::NI;
+  using B::NW;
+  typedef typename Elem<T>::frag frag;
+  static constexpr int kBytesM = BM * 128, kBytesN = BN * 128;  // of one buffer
+
+  // The step buffers, in distinct arrays: the compiler waits for pending
+  // direct loads before an LDS read that may alias their destination.
+  struct Lds {
+    char *m0, *m1, *n0, *n1;
+  };
+
+  Loader<BM, NW, MT> lm;
+  Loader<BN, NW, NT> ln;
+  const char *bm, *bn;
+
+  __device__ __forceinline__ TileProduct(int m0, int n0, int M, int N) : B(m0, n0, M, N) {}
+
+  __device__ __forceinline__ void enter(const SegList& l) {
+    const Seg& s = l.s[this->seg];
+    const int64_t k0 = this->k0;
+    bm = (const char*)s.m + (MT ? k0 * s.ldm + this->m0 : this->m0 * s.ldm + k0) * 2;
+    bn = (const char*)s.n + (NT ? k0 * s.ldn + this->n0 : this->n0 * s.ldn + k0) * 2;
+    lm.enter(this->mrows, s.ldm, this->wave);
+    ln.enter(this->nrows, s.ldn, this->wave);
   }
   // Issue the loads of the current step and move to the next.
   __device__ __forceinline__ void issue(const SegList& l, char* sm, char* sn, bool last) {
-    const int lane = threadIdx.x & 63;
-    const int k = l.s[seg].k;
-    const bool past = k0 + 8 * ((lane & 7) ^ (lane >> 3)) >= k;
-    lm.issue(sm, bm, past, wave);
-    ln.issue(sn, bn, past, wave);
-    k0 += kStepK;
-    bm += kStepK * 2;
-    bn += kStepK * 2;
-    if (k0 >= k && !last) {
-      ++seg;
-      k0 = 0;
+    const int left = l.s[this->seg].k - this->k0;
+    lm.issue(sm, bm, left, this->wave);
+    ln.issue(sn, bn, left, this->wave);
+    this->k0 += 64;
+    bm += lm.step;
+    bn += ln.step;
+    if (left <= 64 && !last) {
+      ++this->seg;
+      this->k0 = 0;
       enter(l);
     }
   }
 
-  __device__ __forceinline__ void multiply(f32x4 (&acc)[MI][NI], const char* sm, const char* sn) const {
+  // Row fragment of rows r0 .. r0 + 15: eight k of row r0 + c, from 32 kk + 8 g.
+  template <int R, bool TURNED>
+  static __device__ __forceinline__ frag read(const char* s, int r0, int kk) {
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-    const char* pm = sm + (wm * MI * 16 + c) * 128;
-    const char* pn = sn + (wn * NI * 16 + c) * 128;
+    if constexpr (!TURNED) {
+      return *(const frag*)(s + (r0 + c) * 128 + 16 * ((4 * kk + g) ^ (c & 7)));
+    } else {
+      const int k = 32 * kk + 8 * g + (c >> 2);  // k + 4 has the same permutation
+      const int col = r0 + 4 * (c & 3);
+      const char* a = s + k * (R * 2) + 16 * ((col >> 3) ^ Loader<R, NW, true>::swz(k)) + 2 * (col & 7);
+      const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(a));
+      const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(a + 4 * R * 2));
+      const i16x4 both[2] = {lo, hi};
+      frag f;
+      __builtin_memcpy(&f, both, 16);
+      return f;
+    }
+  }
+
+  __device__ __forceinline__ void multiply(f32x4 (&acc)[MI][NI], const char* sm, const char* sn) const {
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
-      const int slot = 16 * ((4 * kk + g) ^ (c & 7));
       frag fm[MI], fn[NI];
 #pragma unroll
-      for (int i = 0; i < MI; ++i) fm[i] = *(const frag*)(pm + i * 2048 + slot);
+      for (int i = 0; i < MI; ++i) fm[i] = read<BM, MT>(sm, (this->wm * MI + i) * 16, kk);
 #pragma unroll
-      for (int i = 0; i < NI; ++i) fn[i] = *(const frag*)(pn + i * 2048 + slot);
+      for (int i = 0; i < NI; ++i) fn[i] = read<BN, NT>(sn, (this->wn * NI + i) * 16, kk);
 #pragma unroll
       for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -155,7 +227,8 @@ struct TileProduct {
   // last read of the buffers.
   __device__ __forceinline__ void run(f32x4 (&acc)[MI][NI], const SegList& l, int lo, int hi, const Lds& s) {
     if (lo >= hi) return;  // uniform
-    seek(l, lo);
+    this->seek(l, lo);
+    enter(l);
     issue(l, s.m0, s.n0, lo + 1 >= hi);
     for (int t = lo; t < hi; t += 2) {
       dma_wait();
@@ -170,16 +243,151 @@ struct TileProduct {
     }
     __syncthreads();
   }
+};
 
-  __device__ __forceinline__ static void zero(f32x4 (&acc)[MI][NI]) {
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-      for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+// One fp32 operand's share of a step: 16-byte chunks (eight k of a row) of
+// parts, kTasks per thread.  LDS, per part: [R rows][32 k], chunk ^ (row >> 1 & 3).
+template <int R, int THREADS, bool TURNED>
+struct SplitLoader {
+  static constexpr int kTasks = R * 4 / THREADS;
+  static_assert(kTasks * THREADS == R * 4 && kTasks >= 1, "tile shape");
+  static_assert(!TURNED || kTasks % 2 == 0 || kTasks == 1, "tile shape");
+  static constexpr int kPlane = R * 64;  // bytes of a part's tile
+  float v[kTasks][8];
+
+  // Row and chunk of a task.  plain: four lanes share a row's 128 bytes;
+  // turned: neighbouring lanes have neighbouring rows.
+  static __device__ __forceinline__ int row_of(int t) {
+    const int i = (int)threadIdx.x + t * THREADS;
+    return TURNED ? i % R : i >> 2;
   }
-  // First m (of four) of acc[i][*] and the n of acc[*][j] in this lane.
-  __device__ __forceinline__ int m_of(int i) const { return m0 + (wm * MI + i) * 16 + 4 * ((threadIdx.x & 63) >> 4); }
-  __device__ __forceinline__ int n_of(int j) const { return n0 + (wn * NI + j) * 16 + (threadIdx.x & 15); }
+  static __device__ __forceinline__ int chunk_of(int t) {
+    const int i = (int)threadIdx.x + t * THREADS;
+    return TURNED ? i / R : i & 3;
+  }
+  // base: the tile's first element at this step; rows past valid and k past left are zeros, and so are the k
+  // whose `live` factor is 0 (turned only; live at this step).
+  __device__ __forceinline__ void load(const float* base, int64_t ld, int valid, int left, const float* live) {
+#pragma unroll
+    for (int t = 0; t < kTasks; ++t) {
+      const int r = row_of(t), k = 8 * chunk_of(t);
+      if constexpr (!TURNED) {
+        const float* p = base + r * ld + k;
+        if (r < valid && k + 8 <= left) {
+          __builtin_memcpy(&v[t][0], p, 16);
+          __builtin_memcpy(&v[t][4], p + 4, 16);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[t][j] = r < valid && k + j < left ? p[j] : 0.f;
+        }
+      } else {
+        const float* p = base + k * ld + r;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          v[t][j] = r < valid && k + j < left && (!live || live[k + j] != 0.f) ? p[j * ld] : 0.f;
+      }
+    }
+  }
+  __device__ __forceinline__ void store(char* lds) const {
+#pragma unroll
+    for (int t = 0; t < kTasks; ++t) {
+      const int r = row_of(t), ch = chunk_of(t);
+      u32x4 h, m, l;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t a, b, c;
+        split_pair(v[t][2 * j], v[t][2 * j + 1], a, b, c);
+        h[j] = a;
+        m[j] = b;
+        l[j] = c;
+      }
+      char* p = lds + r * 64 + 16 * (ch ^ ((r >> 1) & 3));
+      *(u32x4*)p = h;
+      *(u32x4*)(p + kPlane) = m;
+      *(u32x4*)(p + 2 * kPlane) = l;
+    }
+  }
+};
+
+template <int BM_, int BN_, int WM_, int WN_, bool MT, bool NT>
+struct SplitProduct : TileBase<BM_, BN_, WM_, WN_, 32> {
+  typedef TileBase<BM_, BN_, WM_, WN_, 32> B;
+  using B::BM;
+  using B::BN;
+  using B::MI;
+  using B::NI;
+  using B::NW;
+  static constexpr int kThreads_ = 64 * NW;
+  static constexpr int kBytesM = BM * 64 * 3, kBytesN = BN * 64 * 3;
+
+  struct Lds {
+    char *m, *n;
+  };
+
+  SplitLoader<BM, kThreads_, MT> lm;
+  SplitLoader<BN, kThreads_, NT> ln;
+  const float* live;  // factors of the k of a turned M operand, or null
+
+  __device__ __forceinline__ SplitProduct(int m0, int n0, int M, int N, const float* live_)
+      : B(m0, n0, M, N), live(live_) {}
+
+  // Load the current step's values and move to the next.
+  __device__ __forceinline__ void load(const SegList& l) {
+    const Seg& s = l.s[this->seg];
+    const int64_t k0 = this->k0;
+    const int left = s.k - this->k0;
+    lm.load((const float*)s.m + (MT ? k0 * s.ldm + this->m0 : this->m0 * s.ldm + k0), s.ldm, this->mrows, left,
+            MT && live ? live + k0 : nullptr);
+    ln.load((const float*)s.n + (NT ? k0 * s.ldn + this->n0 : this->n0 * s.ldn + k0), s.ldn, this->nrows, left,
+            nullptr);
+    this->k0 += 32;
+    if (left <= 32 && this->seg + 1 < l.n) {
+      ++this->seg;
+      this->k0 = 0;
+    }
+  }
+
+  __device__ __forceinline__ void multiply(f32x4 (&acc)[MI][NI], const char* sm, const char* sn) const {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int at = c * 64 + 16 * (g ^ ((c >> 1) & 3));
+    const char* pm = sm + this->wm * MI * 1024 + at;
+    const char* pn = sn + this->wn * NI * 1024 + at;
+    bf16x8 fm[3][MI], fn[3][NI];
+    // part products, the smallest first: (m part, n part)
+    const auto part = [&](int a, int b) {
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) acc[i][j] = Elem<__bf16>::mma(acc[i][j], fm[a][i], fn[b][j]);
+    };
+#pragma unroll
+    for (int a = 2; a >= 0; --a) {
+#pragma unroll
+      for (int i = 0; i < MI; ++i) fm[a][i] = *(const bf16x8*)(pm + a * lm.kPlane + i * 1024);
+#pragma unroll
+      for (int j = 0; j < NI; ++j) fn[a][j] = *(const bf16x8*)(pn + a * ln.kPlane + j * 1024);
+    }
+    part(2, 0);
+    part(0, 2);
+    part(1, 1);
+    part(1, 0);
+    part(0, 1);
+    part(0, 0);
+  }
+
+  __device__ __forceinline__ void run(f32x4 (&acc)[MI][NI], const SegList& l, int lo, int hi, const Lds& s) {
+    if (lo >= hi) return;  // uniform
+    this->seek(l, lo);
+    load(l);
+    for (int t = lo; t < hi; ++t) {
+      lm.store(s.m);
+      ln.store(s.n);
+      __syncthreads();
+      if (t + 1 < hi) load(l);
+      multiply(acc, s.m, s.n);
+      __syncthreads();
+    }
+  }
 };
 
 // Tile (tm, tn) of workgroup `id` among tm_count x tn_count.  Workgroups go to

@@ -5,22 +5,27 @@
 // Everything is tile products (ttt_gemm.h) with work done on the tiles where
 // they are made:
 //   forward    z tiles -> per tile and token (max, sum of exponentials)
-//   backward   z tiles again -> p - 1_t, rounded once to the operand type, in
-//              both orders; then dX = G W and dW = G^T X are plain products
-//   gg         z and U tiles -> h = sum p U; again -> H (and G); then the
-//              products [H|G][W;B] and [H^T|G^T][X;A]
+//   backward   z tiles again -> G = c (p - 1_t); then the products dX = G W
+//              and dW = G^T X
+//   gg         z and U tiles -> H (and G); then [H|G][W;B] and [H^T|G^T][X;A]
 // z is formed again instead of kept: 2 N V d operations against 4 N V bytes
 // written and read.  G and H exist for one piece of the vocabulary at a time
-// (pieces chosen to stay in the 256 MB last-level cache, kPieceBytes).
+// (kPieceBytes), so memory does not grow with N V.
 //
-// fp32 problems run on the bf16 matrix cores: each operand is split into
-// three bf16 parts whose sum is the value, and the six part products above
-// 2^-24 of the whole are summed in fp32, smallest first.  G and H are split
-// the same way where they are made.  An infinity becomes NaN this way.
+// H needs h_i = sum_j p_ij U_ij before its tiles.  As U = A W^T + X B^T,
+//   h_i = A_i . (sum_j p_ij W_j) + X_i . (sum_j p_ij B_j)
+//       = (A_i . dX_i + X_i . (G B)_i) / c_i + U_{i,t_i}
+// where dX is the backward's and G B a product that gX has anyway: a dot
+// product per row in place of a pass over z and U (4 or 6 N V d operations).
+// Only where the upstream gradient's own gradient is asked for (c may be 0
+// there), or dX is not given, are the sums formed from tiles.
 //
-// fp16 holds G and H scaled (kF16Scale, and per row by the largest |U|), since
-// a softmax over a large vocabulary is below fp16's smallest values: powers
-// of two, taken out again in fp32 when the products are stored.
+// 16-bit types: G and H are rounded once to the operands' type, scaled by one
+// factor for all rows (k_factors) that products undo in fp32.  bf16: c over
+// the largest |c|, so that rows which count alike are rounded like p - 1_t
+// itself (one c for all would round the targets' entries, near -c, all to the
+// same side).  fp16: the same with the largest entry at kF16Scale, since a
+// softmax over a large vocabulary is below fp16's smallest values.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <string.h>
@@ -32,82 +37,74 @@
 namespace ttt {
 namespace {
 
-constexpr float kF16Scale = 16384.f;  // of a value in [-1, 1]: the largest power of two with room for sums
+constexpr float kF16Scale = 16384.f;  // the largest stored magnitude: room below fp16's 65504 for rounding
 
-// Eight values to the parts of plane p (PL == 1: rounded to T; PL == 3: the
-// p-th bf16 part of the fp32 value).
-template <typename T, int PL>
-__device__ __forceinline__ uint32_t part_pair(float a, float b, int p) {
-  if constexpr (PL == 1) {
-    typedef T t2 __attribute__((ext_vector_type(2)));
-    const t2 v = __builtin_convertvector(f32x2{a, b}, t2);
-    uint32_t u;
-    __builtin_memcpy(&u, &v, 4);
-    return u;
-  } else {
-    uint32_t h, m, l;
-    split_pair(a, b, h, m, l);
-    return p == 0 ? h : p == 1 ? m : l;
+__host__ __device__ __forceinline__ int round8(int x) { return (x + 7) & ~7; }
+
+// ---------------------------------------------------------------------------
+// Row copies of 16-bit operands: padded to 8 columns (zeros), and zeros in the
+// rows that do not count, which meet factors of 0 in a sum over the rows.
+// ---------------------------------------------------------------------------
+struct CopyArgs {
+  const void* src;  // [R, C], row stride ld
+  int64_t ld;
+  int R, C;
+  void* dst;           // [R][round8(C)]
+  const float* live;   // or null: rows of 0 are left out
+};
+
+__global__ __launch_bounds__(256) void k_copy_rows(CopyArgs a) {
+  const int chunks = round8(a.C) / 8;
+  const int64_t total = (int64_t)a.R * chunks;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int r = (int)(i / chunks), c = 8 * (int)(i % chunks);
+    const uint16_t* s = (const uint16_t*)a.src + (int64_t)r * a.ld + c;
+    uint16_t v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (!a.live || a.live[r] != 0.f) {
+      if (c + 8 <= a.C) {
+        __builtin_memcpy(v, s, 16);
+      } else {
+        for (int j = 0; c + j < a.C; ++j) v[j] = s[j];
+      }
+    }
+    __builtin_memcpy((uint16_t*)a.dst + i * 8, v, 16);
   }
 }
 
 // ---------------------------------------------------------------------------
-// Operand copies: rows padded to 8 columns, parts of fp32, transposes.
+// The products' tile shapes.  16-bit: 256 x 256 (eight waves of 128 x 64) and
+// 128 x 128 (four of 64 x 64); two accumulators: 256 x 128 (eight of 64 x 64)
+// and 128 x 128.  fp32: 128 x 128 (eight of 64 x 32), either way.
 // ---------------------------------------------------------------------------
-struct PackArgs {
-  const void* src;       // [R, C], row stride ld
-  int64_t ld;
-  int R, C;
-  void* rows;            // [PL][R][round8(C)], or null
-  void* cols;            // [PL][C][round8(R)], or null
-  const float* coef;     // rows whose factor is 0 are zeros in `cols`, or null
+template <typename T, bool MT, bool NT, bool DUAL, bool BIG>
+struct ProductOf {
+  static constexpr int BM = BIG ? 256 : 128, BN = BIG && !DUAL ? 256 : 128;
+  static constexpr int WM = DUAL && BIG ? 4 : 2, WN = DUAL && BIG ? 2 : BIG ? 4 : 2;
+  typedef TileProduct<T, BM, BN, WM, WN, MT, NT> type;
+};
+template <bool MT, bool NT, bool DUAL, bool BIG>
+struct ProductOf<float, MT, NT, DUAL, BIG> {
+  typedef SplitProduct<128, 128, 2, 4, MT, NT> type;
 };
 
-__host__ __device__ __forceinline__ int round8(int x) { return (x + 7) & ~7; }
+template <typename T, bool BIG>
+constexpr int kThreadsOf = sizeof(T) == 4 || BIG ? 512 : 256;
 
-// A 64 x 64 tile through LDS.
-template <typename TS, typename T, int PL>
-__global__ __launch_bounds__(256) void k_pack(PackArgs a) {
-  __shared__ float tile[64][65];
-  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
-  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
-  const TS* src = (const TS*)a.src;
-#pragma unroll 4
-  for (int i = y; i < 64; i += 4) {
-    const int r = r0 + i, c = c0 + x;
-    tile[i][x] = r < a.R && c < a.C ? (float)src[(int64_t)r * a.ld + c] : 0.f;
+template <typename T, typename P>
+__device__ __forceinline__ typename P::Lds lds_of() {
+  if constexpr (sizeof(T) == 2) {
+    __shared__ __attribute__((aligned(16))) char m0[P::kBytesM], m1[P::kBytesM], n0[P::kBytesN], n1[P::kBytesN];
+    return {m0, m1, n0, n1};
+  } else {
+    __shared__ __attribute__((aligned(16))) char m[P::kBytesM], n[P::kBytesN];
+    return {m, n};
   }
-  __syncthreads();
-  const int x2 = 2 * (threadIdx.x & 31), y2 = threadIdx.x >> 5;
-  if (a.rows) {
-    const int cp = round8(a.C);
-    const int64_t plane = (int64_t)a.R * cp;
-#pragma unroll 2
-    for (int i = y2; i < 64; i += 8) {
-      const int r = r0 + i, c = c0 + x2;
-      if (r < a.R && c < cp)
-#pragma unroll
-        for (int p = 0; p < PL; ++p)
-          *(uint32_t*)((uint16_t*)a.rows + p * plane + (int64_t)r * cp + c) =
-              part_pair<T, PL>(tile[i][x2], tile[i][x2 + 1], p);
-    }
-  }
-  if (a.cols) {
-    const int rp = round8(a.R);
-    const int64_t plane = (int64_t)a.C * rp;
-    const bool in0 = r0 + x2 < a.R && (!a.coef || a.coef[r0 + x2] != 0.f);
-    const bool in1 = r0 + x2 + 1 < a.R && (!a.coef || a.coef[r0 + x2 + 1] != 0.f);
-#pragma unroll 2
-    for (int i = y2; i < 64; i += 8) {
-      const int c = c0 + i, r = r0 + x2;
-      if (c < a.C && r < rp) {
-        const float v0 = in0 ? tile[x2][i] : 0.f, v1 = in1 ? tile[x2 + 1][i] : 0.f;
-#pragma unroll
-        for (int p = 0; p < PL; ++p)
-          *(uint32_t*)((uint16_t*)a.cols + p * plane + (int64_t)c * rp + r) = part_pair<T, PL>(v0, v1, p);
-      }
-    }
-  }
+}
+
+template <typename T, typename P>
+__device__ __forceinline__ P product_at(int m0, int n0, int M, int N, const float* live) {
+  if constexpr (sizeof(T) == 2) return P(m0, n0, M, N);
+  else return P(m0, n0, M, N, live);
 }
 
 // ---------------------------------------------------------------------------
@@ -122,34 +119,42 @@ struct ZArgs {
   int v0;  // the piece's first vocabulary row
   const int64_t* target;
   const float* stat;  // [N] row max, [N] 1 / sum of exponentials
-  float2* part;       // [parts][N]: (max, sum) | (sum p U, max |U|)
+  float2* part;       // [parts][N]: (max, sum) | (sum p U, -)
   float* at_target;   // [N]: z or U at the target
   const float* h;     // [N]
-  const float *rowmul, *colmul;
-  void *grow, *gcol;  // p - 1_t: [PL][N][round8(M)], [PL][M][round8(N)]
-  void *hrow, *hcol;  // p (U - h)
+  const float* colmul;  // [N]
+  void *g, *hh;       // G and H, [N][round8(M)], or null
 };
 
-// The four-lane-group view of a wave's tile to a [n][m] matrix (rows) and to a
-// [m][n] one (cols), through the wave's own 4 KB of LDS so that global stores
-// are whole 128-byte rows.  val(i, j): the lane's four values of acc[i][j],
-// 0 past M and N.
-template <typename P, typename T, int PL, typename F>
-__device__ __forceinline__ void store_rows(const P& tp, char* lds, void* out, int M, int N, F val) {
-  constexpr int MI = P::MI, NI = P::NI, RB = MI * 32, CH = RB / 16;  // row bytes, chunks
+// A wave's tile to the rows of a [N][round8(M)] matrix.  val(i, j): the lane's
+// four values of acc[i][j], 0 past M.  16-bit: through the wave's own LDS, so
+// that global stores are whole 128-byte rows.
+template <typename P, typename T, typename F>
+__device__ __forceinline__ void store_tile(const P& tp, char* lds, void* out, int M, int N, F val) {
+  constexpr int MI = P::MI, NI = P::NI;
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int ld = round8(M);
-  const int64_t plane = (int64_t)N * ld;
-  char* w = lds + 4096 * tp.wave;
-  for (int p = 0; p < PL; ++p) {
-    T* o = (T*)out + p * plane;
+  T* o = (T*)out;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        const int n = tp.n_of(j), m = tp.m_of(i);
+        const f32x4 v = val(i, j);
+        if (n < N && m < ld) *(f32x4*)(o + (int64_t)n * ld + m) = v;
+      }
+  } else {
+    constexpr int RB = MI * 32, CH = RB / 16;  // row bytes, chunks
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    char* w = lds + 16 * RB * tp.wave;
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
         const f32x4 v = val(i, j);
-        const u32x2 u = {part_pair<T, PL>(v[0], v[1], p), part_pair<T, PL>(v[2], v[3], p)};
-        *(u32x2*)(w + c * RB + 16 * ((2 * i + (g >> 1)) ^ (c & 7)) + 8 * (g & 1)) = u;
+        const t2 u[2] = {__builtin_convertvector(f32x2{v[0], v[1]}, t2), __builtin_convertvector(f32x2{v[2], v[3]}, t2)};
+        __builtin_memcpy(w + c * RB + 16 * ((2 * i + (g >> 1)) ^ (c & 7)) + 8 * (g & 1), u, 8);
       }
 #pragma unroll
       for (int t = 0; t < CH / 4; ++t) {
@@ -162,63 +167,29 @@ __device__ __forceinline__ void store_rows(const P& tp, char* lds, void* out, in
   }
 }
 
-template <typename P, typename T, int PL, typename F>
-__device__ __forceinline__ void store_cols(const P& tp, char* lds, void* out, int M, int N, F val) {
-  constexpr int MI = P::MI, NI = P::NI, RB = NI * 32, CH = RB / 16;
-  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-  const int ld = round8(N);
-  const int64_t plane = (int64_t)M * ld;
-  char* w = lds + 4096 * tp.wave;
-  for (int p = 0; p < PL; ++p) {
-    T* o = (T*)out + p * plane;
-#pragma unroll
-    for (int i = 0; i < MI; ++i) {
-#pragma unroll
-      for (int j = 0; j < NI; ++j) {
-        const f32x4 v = val(i, j);
-        const uint32_t u0 = part_pair<T, PL>(v[0], v[1], p), u1 = part_pair<T, PL>(v[2], v[3], p);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 4 * g + e;
-          *(uint16_t*)(w + r * RB + 16 * ((2 * j + (c >> 3)) ^ (r & (CH - 1))) + 2 * (c & 7)) =
-              (uint16_t)((e < 2 ? u0 : u1) >> (16 * (e & 1)));
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < CH / 4; ++t) {
-        const int r = t * (64 / CH) + lane / CH, ch = lane % CH;
-        const u32x4 u = *(const u32x4*)(w + r * RB + 16 * (ch ^ (r & (CH - 1))));
-        const int m = tp.m0 + (tp.wm * MI + i) * 16 + r, n = tp.n0 + tp.wn * NI * 16 + 8 * ch;
-        if (m < M && n < ld) *(u32x4*)(o + (int64_t)m * ld + n) = u;
-      }
-    }
-  }
-}
-
-template <typename T, int BM, int BN, int WM, int WN, int MODE, int PL>
-__global__ __launch_bounds__(64 * WM * WN) void k_logits(ZArgs a) {
-  typedef TileProduct<T, BM, BN, WM, WN> P;
+template <typename T, int MODE, bool BIG>
+__global__ __launch_bounds__((kThreadsOf<T, BIG>)) void k_logits(ZArgs a) {
+  constexpr bool kDual = MODE >= kHSum;
+  typedef typename ProductOf<T, false, false, kDual, BIG>::type P;
   constexpr int MI = P::MI, NI = P::NI;
-  constexpr bool kDual = MODE == kHSum || MODE == kHGrad;
-  __shared__ __attribute__((aligned(16))) char sm0[BM * 128], sm1[BM * 128], sn0[BN * 128], sn1[BN * 128];
-  static_assert(BM * 128 >= 4096 * WM * WN, "the epilogue's LDS");
-  const typename P::Lds lds{sm0, sm1, sn0, sn1};
+  const typename P::Lds lds = lds_of<T, P>();
   int tm, tn;
   tile_of(blockIdx.x, a.tm, a.tn, &tm, &tn);
-  P tp(tm * BM, tn * BN, a.M, a.N);
+  P tp = product_at<T, P>(tm * P::BM, tn * P::BN, a.M, a.N, nullptr);
   f32x4 z[MI][NI], u[kDual ? MI : 1][kDual ? NI : 1];
   P::zero(z);
-  tp.run(z, a.z, 0, a.z.steps, lds);
+  tp.run(z, a.z, 0, list_steps<P::kStep>(a.z), lds);
   if constexpr (kDual) {
     P::zero(u);
-    tp.run(u, a.u, 0, a.u.steps, lds);
+    tp.run(u, a.u, 0, list_steps<P::kStep>(a.u), lds);
   }
   const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
   for (int j = 0; j < NI; ++j) {
     const int n = tp.n_of(j);
     const bool nin = n < a.N;
-    const int t = nin ? (int)(a.target[n] - a.v0) : -1;  // the target's row in the piece
+    const int64_t td = nin ? a.target[n] - a.v0 : -1;  // the target's row in the piece
+    const int t = td >= 0 && td < a.M ? (int)td : -1;
     if constexpr (MODE == kStats) {
       float mx = -__builtin_inff();
 #pragma unroll
@@ -227,7 +198,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_logits(ZArgs a) {
         for (int e = 0; e < 4; ++e) {
           const int m = tp.m_of(i) + e;
           if (m < a.M) mx = fmaxf(mx, z[i][j][e]);
-          if (m == t && m < a.M) a.at_target[n] = z[i][j][e];
+          if (m == t) a.at_target[n] = z[i][j][e];
         }
       mx = group_max(mx);
       float s = 0.f;
@@ -237,64 +208,47 @@ __global__ __launch_bounds__(64 * WM * WN) void k_logits(ZArgs a) {
         for (int e = 0; e < 4; ++e)
           s += tp.m_of(i) + e < a.M ? fast_exp2((z[i][j][e] - mx) * kLog2e) : 0.f;
       s = group_sum(s);
-      if (g == 0 && nin) a.part[((int64_t)(tm * WM + tp.wm)) * a.N + n] = make_float2(mx, s);
+      if (g == 0 && nin) a.part[((int64_t)(tm * P::WM + tp.wm)) * a.N + n] = make_float2(mx, s);
     } else {
       const float mx = nin ? a.stat[n] : 0.f, inv = nin ? a.stat[a.N + n] : 0.f;
+      const float cm = MODE != kHSum && nin ? a.colmul[n] : 0.f;
       const float h = MODE == kHGrad && nin ? a.h[n] : 0.f;
-      float hs = 0.f, um = 0.f;
+      float hs = 0.f;
 #pragma unroll
       for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int m = tp.m_of(i) + e;
-          const bool in = m < a.M && nin;
-          const float p = in ? fast_exp2((z[i][j][e] - mx) * kLog2e) * inv : 0.f;
-          if constexpr (kDual) {
-            const float uu = u[i][j][e];
-            if constexpr (MODE == kHSum) {
-              hs += in ? p * uu : 0.f;
-              um = fmaxf(um, in ? fabsf(uu) : 0.f);
-              if (in && m == t) a.at_target[n] = uu;
-            } else {
-              u[i][j][e] = in ? p * (uu - h) : 0.f;
-            }
+          // rows of factor 0 are 0 whatever their logits are
+          const bool in = m < a.M && nin && (MODE == kHSum || cm != 0.f);
+          const float p = fast_exp2((z[i][j][e] - mx) * kLog2e) * inv;
+          if constexpr (MODE == kHSum) {
+            hs += in ? p * u[i][j][e] : 0.f;
+            if (m == t) a.at_target[n] = u[i][j][e];
+          } else {
+            if constexpr (MODE == kHGrad) u[i][j][e] = in ? cm * p * (u[i][j][e] - h) : 0.f;
+            z[i][j][e] = in ? cm * (m == t ? p - 1.f : p) : 0.f;
           }
-          z[i][j][e] = in && m == t ? p - 1.f : p;
         }
       if constexpr (MODE == kHSum) {
         hs = group_sum(hs);
-        um = group_max(um);
-        if (g == 0 && nin) a.part[((int64_t)(tm * WM + tp.wm)) * a.N + n] = make_float2(hs, um);
+        if (g == 0 && nin) a.part[((int64_t)(tm * P::WM + tp.wm)) * a.N + n] = make_float2(hs, 0.f);
       }
     }
   }
   if constexpr (MODE == kGrad || MODE == kHGrad) {
-    float rm[NI], cm[NI];
-#pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      const int n = tp.n_of(j);
-      rm[j] = n < a.N ? a.rowmul[n] : 0.f;
-      cm[j] = n < a.N ? a.colmul[n] : 0.f;
-    }
-    // a row of factor 0 is 0 whatever its logits are
-    if (a.grow) store_rows<P, T, PL>(tp, sm0, a.grow, a.M, a.N, [&](int i, int j) { return z[i][j] * rm[j]; });
-    if (a.gcol)
-      store_cols<P, T, PL>(tp, sm0, a.gcol, a.M, a.N, [&](int i, int j) {
-        return cm[j] == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : z[i][j] * cm[j];
-      });
-    if constexpr (kDual) {
-      if (a.hrow) store_rows<P, T, PL>(tp, sm0, a.hrow, a.M, a.N, [&](int i, int j) { return u[i][j] * rm[j]; });
-      if (a.hcol)
-        store_cols<P, T, PL>(tp, sm0, a.hcol, a.M, a.N, [&](int i, int j) {
-          return cm[j] == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : u[i][j] * cm[j];
-        });
-    }
+    char* at;
+    if constexpr (sizeof(T) == 2) at = lds.m0;
+    else at = lds.m;
+    if constexpr (kDual)
+      if (a.hh) store_tile<P, T>(tp, at, a.hh, a.M, a.N, [&](int i, int j) { return u[i][j]; });
+    if (a.g) store_tile<P, T>(tp, at, a.g, a.M, a.N, [&](int i, int j) { return z[i][j]; });
   }
 }
 
 // ---------------------------------------------------------------------------
-// Plain products: out[n][m] = mul[n] * alpha * sum_k, to the output, or as
-// fp32 to part[split][N][M] (added to what is there from earlier pieces).
+// Plain products: out[n][m] = alpha * sum_k, to the output (and its fp32 copy),
+// or as fp32 to part[split][N][M] (added to what is there from earlier pieces).
 // ---------------------------------------------------------------------------
 struct OutArgs {
   SegList l;
@@ -304,67 +258,74 @@ struct OutArgs {
   int add;
   void* out;
   int64_t ld;
-  const float* mul;    // [N] or null; a row of factor 0 is 0
-  const float* alpha;  // one value or null
+  float* out32;       // [N][M] or null
+  const float* rows;  // [N] or null: rows that do not count (0) are 0
+  const float* live;  // turned fp32 M operand: the k that do not count are left out
+  const float* alpha;
 };
 
-template <typename T, typename TO, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void k_product(OutArgs a) {
-  typedef TileProduct<T, BM, BN, WM, WN> P;
+template <typename T, bool NT, bool BIG>
+__global__ __launch_bounds__((kThreadsOf<T, BIG>)) void k_product(OutArgs a) {
+  typedef typename ProductOf<T, true, NT, false, BIG>::type P;
   constexpr int MI = P::MI, NI = P::NI;
-  __shared__ __attribute__((aligned(16))) char sm0[BM * 128], sm1[BM * 128], sn0[BN * 128], sn1[BN * 128];
-  const typename P::Lds lds{sm0, sm1, sn0, sn1};
+  const typename P::Lds lds = lds_of<T, P>();
   const int s = blockIdx.x / (a.tm * a.tn), id = blockIdx.x % (a.tm * a.tn);
   int tm, tn;
   tile_of(id, a.tm, a.tn, &tm, &tn);
-  P tp(tm * BM, tn * BN, a.M, a.N);
+  P tp = product_at<T, P>(tm * P::BM, tn * P::BN, a.M, a.N, a.live);
   f32x4 acc[MI][NI];
   P::zero(acc);
-  const int lo = s * a.chunk, hi = lo + a.chunk < a.l.steps ? lo + a.chunk : a.l.steps;
+  const int steps = list_steps<P::kStep>(a.l), lo = s * a.chunk, hi = lo + a.chunk < steps ? lo + a.chunk : steps;
   tp.run(acc, a.l, lo, hi, lds);
-  const float al = a.part || !a.alpha ? 1.f : *a.alpha;
+  const float al = a.part ? 1.f : *a.alpha;
 #pragma unroll
   for (int j = 0; j < NI; ++j) {
     const int n = tp.n_of(j);
     if (n >= a.N) continue;
-    const float mul = (a.part || !a.mul ? 1.f : a.mul[n]) * al;
+    const bool dead = !a.part && a.rows && a.rows[n] == 0.f;
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
       const int m = tp.m_of(i);
       if (m >= a.M) continue;
+      const int cnt = a.M - m < 4 ? a.M - m : 4;
       f32x4 v = acc[i][j];
       if (a.part) {
         float* o = a.part + ((int64_t)s * a.N + n) * a.M + m;
-        if (m + 4 <= a.M) {
+        if (cnt == 4) {
           f32x4 old = {0.f, 0.f, 0.f, 0.f};
           if (a.add) __builtin_memcpy(&old, o, 16);
           v += old;
           __builtin_memcpy(o, &v, 16);
         } else {
-          for (int e = 0; m + e < a.M; ++e) o[e] = a.add ? o[e] + v[e] : v[e];
+          for (int e = 0; e < cnt; ++e) o[e] = a.add ? o[e] + v[e] : v[e];
         }
       } else {
-        v = mul == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : v * mul;
-        TO* o = (TO*)a.out + (int64_t)n * a.ld + m;
-        if (m + 4 <= a.M) {
-          TO r[4] = {(TO)v[0], (TO)v[1], (TO)v[2], (TO)v[3]};
+        v = dead ? f32x4{0.f, 0.f, 0.f, 0.f} : v * al;
+        T* o = (T*)a.out + (int64_t)n * a.ld + m;
+        float* o32 = a.out32 ? a.out32 + (int64_t)n * a.M + m : nullptr;
+        if (cnt == 4) {
+          const T r[4] = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
           __builtin_memcpy(o, r, sizeof(r));
+          if (o32) __builtin_memcpy(o32, &v, 16);
         } else {
-          for (int e = 0; m + e < a.M; ++e) o[e] = (TO)v[e];
+          for (int e = 0; e < cnt; ++e) {
+            o[e] = (T)v[e];
+            if (o32) o32[e] = v[e];
+          }
         }
       }
     }
   }
 }
 
-// out[n][m] = mul[n] * alpha * sum of the splits' parts, in their order.
-template <typename TO>
+// out[n][m] = alpha * sum of the splits' parts, in their order.
+template <typename T>
 __global__ __launch_bounds__(256) void k_finish(OutArgs a) {
   const int64_t total = (int64_t)a.N * a.M, i4 = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i4 >= total) return;
-  const float al = a.alpha ? *a.alpha : 1.f;
-  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  const float al = *a.alpha;
   const int cnt = total - i4 < 4 ? (int)(total - i4) : 4;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
   for (int s = 0; s < a.split; ++s) {
     const float* p = a.part + s * total + i4;
     if (cnt == 4) {
@@ -375,10 +336,22 @@ __global__ __launch_bounds__(256) void k_finish(OutArgs a) {
       for (int e = 0; e < cnt; ++e) v[e] += p[e];
     }
   }
+  int n = (int)(i4 / a.M), m = (int)(i4 % a.M);
+  if (cnt == 4 && m + 4 <= a.M) {
+    v = a.rows && a.rows[n] == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : v * al;
+    const T r[4] = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+    __builtin_memcpy((T*)a.out + n * a.ld + m, r, sizeof(r));
+    if (a.out32) __builtin_memcpy(a.out32 + i4, &v, 16);
+    return;
+  }
   for (int e = 0; e < cnt; ++e) {
-    const int64_t n = (i4 + e) / a.M, m = (i4 + e) % a.M;
-    const float mul = (a.mul ? a.mul[n] : 1.f) * al;
-    ((TO*)a.out)[n * a.ld + m] = (TO)(mul == 0.f ? 0.f : v[e] * mul);
+    const float r = a.rows && a.rows[n] == 0.f ? 0.f : v[e] * al;
+    ((T*)a.out)[n * a.ld + m] = (T)r;
+    if (a.out32) a.out32[i4 + e] = r;
+    if (++m == a.M) {
+      m = 0;
+      ++n;
+    }
   }
 }
 
@@ -386,7 +359,7 @@ __global__ __launch_bounds__(256) void k_finish(OutArgs a) {
 // Row kernels.
 // ---------------------------------------------------------------------------
 struct RowArgs {
-  int N, V, parts, reduction, f16;
+  int N, V, parts, reduction, dtype;
   int64_t ignore;
   const int64_t* target;
   const float* weight;  // row weights or null
@@ -397,8 +370,8 @@ struct RowArgs {
   float* row;   // [N]: the rows' losses | the rows' shares of the upstream gradient's gradient
   float* out;   // reduced
   float* h;
-  float* umax;
-  float *coef, *rowmul, *colmul, *outmul, *alpha;
+  float *coef, *live, *colmul, *alpha;
+  const float *nx, *na, *nw, *nb;  // row norms of X, A, W, B (fp16 gg), or null
 };
 
 __device__ __forceinline__ float row_weight(const RowArgs& a, int n) {
@@ -406,47 +379,73 @@ __device__ __forceinline__ float row_weight(const RowArgs& a, int n) {
 }
 __device__ __forceinline__ bool bad_target(const RowArgs& a, int n) { return a.target[n] < 0 || a.target[n] >= a.V; }
 
+// (max, sum of exponentials about it) of two sets.
+__device__ __forceinline__ float2 join_stats(float2 a, float2 b) {
+  const float mx = fmaxf(a.x, b.x);
+  return make_float2(mx, (a.y == 0.f ? 0.f : a.y * fast_exp2((a.x - mx) * kLog2e)) +
+                             (b.y == 0.f ? 0.f : b.y * fast_exp2((b.x - mx) * kLog2e)));
+}
+
+// The parts' results of 64 tokens a workgroup, its sixteen waves taking a
+// part each in turn; to wave 0.
+template <bool STATS>
+__device__ __forceinline__ float2 join_parts(const float2* part, int parts, int N, int n, float2 (*lds)[64]) {
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  float2 s = make_float2(STATS ? -__builtin_inff() : 0.f, 0.f);
+  if (n < N)
+#pragma unroll 4
+    for (int i = w; i < parts; i += 16) {
+      const float2 p = part[(int64_t)i * N + n];
+      if constexpr (STATS) s = join_stats(s, p);
+      else s.x += p.x;
+    }
+  lds[w][lane] = s;
+  __syncthreads();
+  if (w == 0)
+    for (int i = 1; i < 16; ++i) {
+      if constexpr (STATS) s = join_stats(s, lds[i][lane]);
+      else s.x += lds[i][lane].x;
+    }
+  return s;
+}
+
 // The tiles' (max, sum) to the row's, and its loss: log(sum) - (z_t - max),
 // which keeps its digits where the target has nearly all of the probability.
-__global__ __launch_bounds__(256) void k_join_loss(RowArgs a) {
-  const int n = blockIdx.x * 256 + threadIdx.x;
-  if (n >= a.N) return;
-  float mx = -__builtin_inff(), s = 0.f;
-  for (int i = 0; i < a.parts; ++i) mx = fmaxf(mx, a.part[(int64_t)i * a.N + n].x);
-  for (int i = 0; i < a.parts; ++i) {
-    const float2 p = a.part[(int64_t)i * a.N + n];
-    s += p.y == 0.f ? 0.f : p.y * fast_exp2((p.x - mx) * kLog2e);
-  }
-  a.stat[n] = mx;
-  a.stat[a.N + n] = 1.f / s;
+__global__ __launch_bounds__(1024) void k_join_loss(RowArgs a) {
+  __shared__ float2 lds[16][64];
+  const int n = blockIdx.x * 64 + (threadIdx.x & 63);
+  const float2 s = join_parts<true>(a.part, a.parts, a.N, n, lds);
+  if (threadIdx.x >= 64 || n >= a.N) return;
+  a.stat[n] = s.x;
+  a.stat[a.N + n] = 1.f / s.y;
   const float w = row_weight(a, n);
-  const float l = bad_target(a, n) ? __builtin_nanf("") : logf(s) - (a.at_target[n] - mx);
+  const float l = bad_target(a, n) ? __builtin_nanf("") : logf(s.y) - (a.at_target[n] - s.x);
   a.row[n] = w == 0.f ? 0.f : w * l;
+}
+
+// h = sum p U, and the rows' shares of the upstream gradient's gradient.
+__global__ __launch_bounds__(1024) void k_join_h(RowArgs a) {
+  __shared__ float2 lds[16][64];
+  const int n = blockIdx.x * 64 + (threadIdx.x & 63);
+  const float2 s = join_parts<false>(a.part, a.parts, a.N, n, lds);
+  if (threadIdx.x >= 64 || n >= a.N) return;
+  a.h[n] = s.x;
+  if (a.row) {
+    const float w = row_weight(a, n);
+    a.row[n] = w == 0.f ? 0.f
+               : bad_target(a, n) ? __builtin_nanf("")
+                                  : w * a.stat[2 * a.N] * (s.x - a.at_target[n]);
+  }
 }
 
 // Rows 0 .. parts - 1 of the tiles' partial results to row 0, so that what is
 // kept does not grow with the vocabulary.
-template <int MODE>
-__global__ __launch_bounds__(256) void k_merge(float2* part, int parts, int N) {
-  const int n = blockIdx.x * 256 + threadIdx.x;
-  if (n >= N) return;
-  if constexpr (MODE == kStats) {
-    float mx = -__builtin_inff(), s = 0.f;
-    for (int i = 0; i < parts; ++i) mx = fmaxf(mx, part[(int64_t)i * N + n].x);
-    for (int i = 0; i < parts; ++i) {
-      const float2 p = part[(int64_t)i * N + n];
-      s += p.y == 0.f ? 0.f : p.y * fast_exp2((p.x - mx) * kLog2e);
-    }
-    part[n] = make_float2(mx, s);
-  } else {
-    float s = 0.f, um = 0.f;
-    for (int i = 0; i < parts; ++i) {
-      const float2 p = part[(int64_t)i * N + n];
-      s += p.x;
-      um = fmaxf(um, p.y);
-    }
-    part[n] = make_float2(s, um);
-  }
+template <bool STATS>
+__global__ __launch_bounds__(1024) void k_merge(float2* part, int parts, int N) {
+  __shared__ float2 lds[16][64];
+  const int n = blockIdx.x * 64 + (threadIdx.x & 63);
+  const float2 s = join_parts<STATS>(part, parts, N, n, lds);
+  if (threadIdx.x < 64 && n < N) part[n] = s;
 }
 
 // A workgroup's sum in a fixed order.
@@ -460,12 +459,23 @@ __device__ __forceinline__ float block_sum(float v, float* lds) {
   for (int i = 0; i < (int)(blockDim.x >> 6); ++i) t += lds[i];
   return t;
 }
+__device__ __forceinline__ float block_max(float v, float* lds) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) v = fmaxf(v, __shfl_xor(v, m));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float t = lds[0];
+  for (int i = 1; i < (int)(blockDim.x >> 6); ++i) t = fmaxf(t, lds[i]);
+  return t;
+}
 
 // One workgroup: the rows' losses and weights to the loss and its denominator.
 __global__ __launch_bounds__(1024) void k_reduce_loss(RowArgs a) {
   __shared__ float lds[16];
   float l = 0.f, w = 0.f;
   if (a.reduction != TTT_REDUCE_NONE)
+#pragma unroll 4
     for (int n = threadIdx.x; n < a.N; n += 1024) {
       l += a.row[n];
       w += row_weight(a, n);
@@ -480,66 +490,47 @@ __global__ __launch_bounds__(1024) void k_reduce_loss(RowArgs a) {
   }
 }
 
-// The rows' coefficients c and the factors that G is stored with.  fp16: one
-// workgroup, which finds the largest |c| (times the row's scale) first.
+// The rows' coefficients c, which rows count, and the factors that G and H are stored with:
+// colmul, undone by alpha.  One workgroup for 16-bit types: it finds the
+// largest |c| (fp16 gg: times a bound of the row's |U - h|, 2 max |U| <= 2
+// (|A_i| max |W_j| + |X_i| max |B_j|)) first.
 __global__ __launch_bounds__(1024) void k_factors(RowArgs a) {
   __shared__ float lds[16];
   const float inv = a.stat[2 * a.N];
-  float top = 0.f;
+  float wm = 0.f, bm = 0.f, top = 0.f;
+  if (a.nw || a.nb) {
+    for (int v = threadIdx.x; v < a.V; v += 1024) {
+      if (a.nw) wm = fmaxf(wm, a.nw[v]);
+      if (a.nb) bm = fmaxf(bm, a.nb[v]);
+    }
+    wm = block_max(wm, lds);
+    bm = block_max(bm, lds);
+  }
   const int stride = gridDim.x * 1024;
+#pragma unroll 2
   for (int n = blockIdx.x * 1024 + threadIdx.x; n < a.N; n += stride) {
     const float w = row_weight(a, n);
     const float up = a.grad_loss[a.reduction == TTT_REDUCE_NONE ? n : 0];
     const float c = w == 0.f ? 0.f : bad_target(a, n) ? __builtin_nanf("") : up * w * inv;
     a.coef[n] = c;
-    if (!a.f16) {
-      a.rowmul[n] = 1.f;
-      a.colmul[n] = a.outmul[n] = c;
-    } else {
-      // |p (U - h)| <= 2 max |U|: a power of two that keeps it (and p) below kF16Scale
-      int e = 0;
-      if (a.umax) (void)frexpf(fmaxf(1.f, 2.f * a.umax[n]), &e);
-      const float rm = ldexpf(kF16Scale, -e);
-      a.rowmul[n] = rm;
-      a.outmul[n] = c / rm;
-      const float t = fabsf(c / rm);
-      if (t < __builtin_inff()) top = fmaxf(top, t);
+    a.live[n] = w == 0.f ? 0.f : 1.f;
+    if (a.dtype == TTT_F32) a.colmul[n] = c;
+    float t = fabsf(c);
+    if (a.nw || a.nb) {
+      const float ub = (a.na ? a.na[n] * wm : 0.f) + (a.nb ? a.nx[n] * bm : 0.f);
+      t *= fmaxf(1.f, 2.f * ub);
     }
+    if (c != 0.f && t < __builtin_inff()) top = fmaxf(top, t);
   }
-  if (!a.f16) {
+  if (a.dtype == TTT_F32) {
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.alpha = 1.f;
     return;
   }
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = top;
-  __syncthreads();
-  for (int i = 0; i < 16; ++i) top = fmaxf(top, lds[i]);
-  int e = 0;
-  (void)frexpf(top, &e);
-  e = top == 0.f ? 0 : e > 120 ? 120 : e < -120 ? -120 : e;
-  // c 2^-e / rm <= 1: the largest stored |value| is the row's own bound
-  for (int n = threadIdx.x; n < a.N; n += 1024) a.colmul[n] = ldexpf(a.coef[n], -e);
-  if (threadIdx.x == 0) *a.alpha = ldexpf(1.f, e);
-}
-
-__global__ __launch_bounds__(256) void k_join_h(RowArgs a) {
-  const int n = blockIdx.x * 256 + threadIdx.x;
-  if (n >= a.N) return;
-  float s = 0.f, um = 0.f;
-  for (int i = 0; i < a.parts; ++i) {
-    const float2 p = a.part[(int64_t)i * a.N + n];
-    s += p.x;
-    um = fmaxf(um, p.y);
-  }
-  a.h[n] = s;
-  if (a.umax) a.umax[n] = um;
-  if (a.row) {
-    const float w = row_weight(a, n);
-    a.row[n] = w == 0.f ? 0.f
-               : bad_target(a, n) ? __builtin_nanf("")
-                                  : w * a.stat[2 * a.N] * (s - a.at_target[n]);
-  }
+  top = fmaxf(block_max(top, lds), 1e-30f);
+  const float s = (a.dtype == TTT_F16 ? kF16Scale : 1.f) / top;
+#pragma unroll 2
+  for (int n = threadIdx.x; n < a.N; n += 1024) a.colmul[n] = a.coef[n] * s;
+  if (threadIdx.x == 0) *a.alpha = a.dtype == TTT_F16 ? top * (1.f / kF16Scale) : top;
 }
 
 __global__ __launch_bounds__(1024) void k_sum(const float* x, int n, float* out) {
@@ -550,41 +541,103 @@ __global__ __launch_bounds__(1024) void k_sum(const float* x, int n, float* out)
   if (threadIdx.x == 0) *out = s;
 }
 
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+  return v;
+}
+
+// norm[r] = |row r|, a wave a row.
+template <typename T>
+__global__ __launch_bounds__(256) void k_norms(const T* x, int64_t ld, int R, int C, float* norm) {
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (r >= R) return;
+  float s = 0.f;
+  for (int c = lane; c < C; c += 64) {
+    const float v = (float)x[r * ld + c];
+    s += v * v;
+  }
+  s = wave_sum(s);
+  if (lane == 0) norm[r] = sqrtf(s);
+}
+
+struct HArgs {
+  int N, V, d, split;
+  const int64_t* target;
+  const float *coef, *alpha;
+  const void *x, *w, *a, *b;  // a, b: or null
+  int64_t ldx, ldw, lda, ldb;
+  const float* dx32;  // [N][d]: the backward's dX (with a)
+  const float* gb;    // [split][N][d]: G B (with b), over alpha
+  float* h;
+};
+
+// h_i = (A_i . dX_i + X_i . (G B)_i) / c_i + A_i . W_t + X_i . B_t: a wave a row.
+template <typename T>
+__global__ __launch_bounds__(256) void k_row_h(HArgs a) {
+  const int n = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (n >= a.N) return;
+  const float c = a.coef[n];
+  if (!(c != 0.f) || c != c) {  // uniform: a row that does not count, or a target that does not exist
+    if (lane == 0) a.h[n] = 0.f;
+    return;
+  }
+  const int64_t t = a.target[n], n64 = n;
+  const float al = *a.alpha;
+  float s = 0.f, u = 0.f;
+  for (int i = lane; i < a.d; i += 64) {
+    if (a.a) {
+      const float v = (float)((const T*)a.a)[n64 * a.lda + i];
+      s += v * a.dx32[n64 * a.d + i];
+      u += v * (float)((const T*)a.w)[t * a.ldw + i];
+    }
+    if (a.b) {
+      const float v = (float)((const T*)a.x)[n64 * a.ldx + i];
+      float q = 0.f;
+      for (int k = 0; k < a.split; ++k) q += a.gb[((int64_t)k * a.N + n64) * a.d + i];
+      s += v * (q * al);
+      u += v * (float)((const T*)a.b)[t * a.ldb + i];
+    }
+  }
+  s = wave_sum(s);
+  u = wave_sum(u);
+  if (lane == 0) a.h[n] = s / c + u;
+}
+
 // ---------------------------------------------------------------------------
 // Host: sizes, workspace layout, launches.
 // ---------------------------------------------------------------------------
-constexpr int64_t kPieceBytes = 128ll << 20;  // G (and H) of a piece, all orders and parts
-constexpr int64_t kPackBytes = 256ll << 20;   // packed head rows of a forward piece
+constexpr int64_t kPieceBytes = 512ll << 20;  // G (and H) of a piece
+constexpr int64_t kPackBytes = 256ll << 20;   // copied head rows of a forward piece
 constexpr int kMaxSplit = 16;
 constexpr int kMaxParts = 1024;    // rows of the tiles' partial results that are kept before they are merged
-constexpr int kStatsRows = 32768;  // vocabulary rows of a forward piece: at most kMaxParts / 2 such rows
-
-struct Plan {
-  int dtype, entry, PL, N, V, d, dp, Np;
-  bool f32, pack;  // pack: rows are copied (parts of fp32, or not a multiple of 8 columns)
-  int vc, pieces;  // vocabulary rows of a piece
-};
+constexpr int kStatsRows = 32768;  // vocabulary rows of a piece: at most kMaxParts / 2 such rows
 
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+struct Plan {
+  int dtype, entry, N, V, d, dp, es;
+  bool f32, pack;  // pack: 16-bit rows are copied (not a multiple of 8 columns)
+  int vc, pieces;  // vocabulary rows of a piece
+};
 
 Plan plan_of(const ttt_lce_problem* p, int entry) {
   Plan k;
   k.dtype = p->dtype;
   k.entry = entry;
   k.f32 = p->dtype == TTT_F32;
-  k.PL = k.f32 ? 3 : 1;
+  k.es = k.f32 ? 4 : 2;
   k.N = (int)p->rows;
   k.V = (int)p->vocab;
   k.d = (int)p->cols;
   k.dp = round8(k.d);
-  k.Np = round8(k.N);
-  k.pack = k.f32 || k.d % 8 != 0;
+  k.pack = !k.f32 && k.d % 8 != 0;
   int64_t vc = kStatsRows;
   if (entry == TTT_LCE_FWD) {
-    const int64_t fit = kPackBytes / ((int64_t)k.dp * k.PL * 2);
+    const int64_t fit = kPackBytes / ((int64_t)k.dp * 2);
     if (k.pack && fit < vc) vc = fit;
   } else {
-    vc = kPieceBytes / ((int64_t)k.Np * k.PL * 2 * (entry == TTT_LCE_BWD ? 2 : 4));
+    vc = kPieceBytes / ((int64_t)k.N * k.es * (entry == TTT_LCE_BWD ? 1 : 2));
   }
   vc = vc / 256 * 256;
   if (vc < 256) vc = 256;
@@ -615,31 +668,45 @@ struct Spread {  // the tiles of a product and the workgroups of each
   int tm, tn, split, chunk;
 };
 
-Spread spread_of(int M, int N, int steps) {
-  Spread s;
-  s.big = cdiv(M, 256) * cdiv(N, 256) >= 192;
-  const int b = s.big ? 256 : 128;
-  s.tm = (int)cdiv(M, b);
-  s.tn = (int)cdiv(N, b);
-  const int64_t tiles = (int64_t)s.tm * s.tn, want = s.big ? 256 : 512;
-  int64_t split = tiles >= want / 2 ? 1 : cdiv(want, tiles);
-  if (split > kMaxSplit) split = kMaxSplit;
-  if (split > steps / 4) split = steps / 4 < 1 ? 1 : steps / 4;
-  s.chunk = (int)cdiv(steps, split);
-  s.split = (int)cdiv(steps, s.chunk);
-  return s;
+// The tile shape and split of a plain product of k in `segs` segments: the
+// least of (rounds of workgroups) x (steps of each) x (a step's time), plus the
+// parts' traffic where they are split.  Steps (us) at full occupancy, measured
+// on products that fill the card.
+Spread spread_of(const Plan& p, int M, int N, int64_t k, bool keep) {
+  const int step = p.f32 ? 32 : 64;
+  const int steps = (int)cdiv(k, step);
+  Spread best{false, 0, 0, 0, 0};
+  double least = 1e30;
+  for (int big = 0; big < (p.f32 ? 1 : 2); ++big) {
+    const int b = big ? 256 : 128, slots = big ? 256 : 512;
+    const double us = p.f32 ? 2.2 : big ? 1.8 : 1.4;
+    const int tm = (int)cdiv(M, b), tn = (int)cdiv(N, b);
+    for (int split = 1; split <= kMaxSplit; split += split < 4 ? 1 : 2) {
+      if (split > 1 && split * 4 > steps) break;
+      const int chunk = (int)cdiv(steps, split);
+      const double rounds = (double)cdiv((int64_t)tm * tn * split, slots);
+      double t = rounds * (chunk * us + 3);
+      if (split > 1 || keep) t += 4 + 8.0 * split * M * N / 4e6;
+      if (t < least) {
+        least = t;
+        best = Spread{big != 0, tm, tn, (int)cdiv(steps, chunk), chunk};
+      }
+    }
+  }
+  return best;
 }
 
-int steps_of(int k) { return (k + kStepK - 1) / kStepK; }
+// Of the products over a piece's vocabulary, [N, d], and over the tokens,
+// [vc, d], with `segs` segments.
+Spread spread_x(const Plan& k, int segs, bool keep) { return spread_of(k, k.d, k.N, (int64_t)segs * k.vc, keep); }
+Spread spread_w(const Plan& k, int segs) { return spread_of(k, k.d, k.vc, (int64_t)segs * k.N, false); }
 
 struct Buffers {
-  // operand copies
-  void *xr, *xt, *ar, *at;  // x and a: rows, transposed
-  void *wr, *wt, *br, *bt;  // of the piece of w and b
-  void *grow, *gcol, *hrow, *hcol;
-  float *part_x, *part_w;   // fp32 parts of dx, dw
+  void *xr, *ar, *wr, *br;  // row copies
+  void *g, *hh;
+  float *part_x, *part_w;  // fp32 parts of dx, dw
   float2* part;
-  float *at_target, *row, *h, *umax, *coef, *rowmul, *colmul, *outmul, *alpha;
+  float *at_target, *row, *h, *coef, *live, *colmul, *alpha, *nx, *na, *nw, *nb;
   int parts;
 };
 
@@ -647,155 +714,141 @@ struct Buffers {
 Buffers layout(const Plan& k, Carver* c) {
   Buffers b;
   memset(&b, 0, sizeof(b));
-  const int64_t e = 2 * k.PL;
-  const int vcp = round8(k.vc);
   const bool fwd = k.entry == TTT_LCE_FWD, gg = k.entry == TTT_LCE_GG;
-  const int64_t each = cdiv(k.vc, 128) * 2;
-  if (fwd || gg) b.parts = (int)(each * k.pieces < kMaxParts ? each * k.pieces : kMaxParts);
+  const int64_t each = cdiv(k.vc, 128) * 4;
+  if (fwd || gg) b.parts = (int)(each * k.pieces < each + kMaxParts ? each * k.pieces : each + kMaxParts);
   if (b.parts) b.part = (float2*)c->take((int64_t)b.parts * k.N * 8);
   b.at_target = c->floats(k.N);
   b.row = c->floats(k.N);
-  if (k.pack) {
-    b.xr = c->take(e * k.N * k.dp);
-    b.wr = c->take(e * k.vc * k.dp);
-    if (gg) {
-      b.ar = c->take(e * k.N * k.dp);
-      b.br = c->take(e * k.vc * k.dp);
+  if (!k.f32) {
+    const int64_t xb = 2 * (int64_t)k.N * k.dp;
+    if (k.pack || !fwd) b.xr = c->take(xb);
+    if (gg) b.ar = c->take(xb);
+    if (k.pack) {
+      b.wr = c->take(2 * (int64_t)k.vc * k.dp);
+      if (gg) b.br = c->take(2 * (int64_t)k.vc * k.dp);
     }
   }
   if (fwd) return b;
   b.h = c->floats(k.N);
-  b.umax = c->floats(k.N);
   b.coef = c->floats(k.N);
-  b.rowmul = c->floats(k.N);
+  b.live = c->floats(k.N);
   b.colmul = c->floats(k.N);
-  b.outmul = c->floats(k.N);
   b.alpha = c->floats(1);
-  b.xt = c->take(e * k.d * k.Np);
-  b.wt = c->take(e * k.d * vcp);
-  b.grow = c->take(e * k.N * vcp);
-  b.gcol = c->take(e * k.vc * k.Np);
+  const int64_t gb = (int64_t)k.es * k.N * round8(k.vc);
+  b.g = c->take(gb);
   if (gg) {
-    b.at = c->take(e * k.d * k.Np);
-    b.bt = c->take(e * k.d * vcp);
-    b.hrow = c->take(e * k.N * vcp);
-    b.hcol = c->take(e * k.vc * k.Np);
+    b.hh = c->take(gb);
+    if (k.dtype == TTT_F16) {
+      b.nx = c->floats(k.N);
+      b.na = c->floats(k.N);
+      b.nw = c->floats(k.V);
+      b.nb = c->floats(k.V);
+    }
   }
   // parts: the most that any set of segments asks for
-  const int terms = k.f32 ? 6 : 1, most = gg ? 2 : 1;
   int64_t px = 0, pw = 0;
-  for (int n = 1; n <= most; ++n) {
-    const Spread sx = spread_of(k.d, k.N, n * terms * steps_of(vcp));
-    const Spread sw = spread_of(k.d, k.vc, n * terms * steps_of(k.Np));
-    if (sx.split > px) px = sx.split;
-    if (sw.split > pw) pw = sw.split;
+  for (int n = 1; n <= (gg ? 2 : 1); ++n) {
+    for (int keep = 0; keep < 2; ++keep) {
+      const int s = spread_x(k, n, keep).split;
+      if (s > px) px = s;
+    }
+    const int s = spread_w(k, n).split;
+    if (s > pw) pw = s;
   }
   b.part_x = c->floats(px * k.N * k.d);
   b.part_w = c->floats(pw * k.vc * k.d);
   return b;
 }
 
-// The products of parts of an fp32 product, smallest first: (m part, n part).
-const int kTerms[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
-
-// Adds the product of two packed (or 16-bit) operands over k to the list.
-void add_product(SegList* l, const Plan& pl, const void* m, int64_t ldm, int64_t planem, const void* n, int64_t ldn,
-                 int64_t planen, int k) {
-  const int terms = pl.f32 ? 6 : 1;
-  for (int t = 0; t < terms; ++t) {
-    const int pm = pl.f32 ? kTerms[t][0] : 0, pn = pl.f32 ? kTerms[t][1] : 0;
-    Seg& s = l->s[l->n++];
-    s.m = (const char*)m + 2 * planem * pm;
-    s.n = (const char*)n + 2 * planen * pn;
-    s.ldm = ldm;
-    s.ldn = ldn;
-    s.k = k;
-    l->steps += steps_of(k);
-  }
-}
-
 struct Operand {
   const void* p;
-  int64_t ld, plane;
+  int64_t ld;
 };
 
-void launch_pack(const Plan& k, const void* src, int64_t ld, int R, int C, void* rows, void* cols, const float* coef,
-                 hipStream_t st) {
-  if (!rows && !cols) return;
-  PackArgs a{src, ld, R, C, rows, cols, coef};
-  // the padded columns of `rows` and rows of `cols` lie in the last tiles
-  const dim3 grid((unsigned)cdiv(C, 64), (unsigned)cdiv(R, 64));
-  if (k.dtype == TTT_F32) k_pack<float, __bf16, 3><<<grid, 256, 0, st>>>(a);
-  else if (k.dtype == TTT_BF16) k_pack<__bf16, __bf16, 1><<<grid, 256, 0, st>>>(a);
-  else k_pack<_Float16, _Float16, 1><<<grid, 256, 0, st>>>(a);
+void add_product(SegList* l, Operand m, Operand n, int k) {
+  Seg& s = l->s[l->n++];
+  s.m = m.p;
+  s.n = n.p;
+  s.ldm = m.ld;
+  s.ldn = n.ld;
+  s.k = k;
+}
+
+void launch_copy(const void* src, int64_t ld, int R, int C, void* dst, const float* live, hipStream_t st) {
+  CopyArgs a{src, ld, R, C, dst, live};
+  const int64_t n = cdiv((int64_t)R * (round8(C) / 8), 256);
+  k_copy_rows<<<(unsigned)(n < 8192 ? n : 8192), 256, 0, st>>>(a);
+}
+
+// Tiles of 256 where there are enough of them to fill the card.
+bool big_logits(const Plan& k, bool dual, int M, int N) {
+  return !k.f32 && cdiv(M, 256) * cdiv(N, dual ? 128 : 256) >= 192;
+}
+
+// Rows of parts that launch_logits writes for M vocabulary rows: one per wave
+// along them.
+int parts_of(const Plan& k, bool dual, int M, int N) {
+  const bool big = big_logits(k, dual, M, N);
+  return (int)cdiv(M, big ? 256 : 128) * (big && dual ? 4 : 2);
 }
 
 template <int MODE>
 void launch_logits(const Plan& k, ZArgs a, hipStream_t st) {
-  constexpr bool dual = MODE == kHSum || MODE == kHGrad;
-  const bool big = !dual && cdiv(a.M, 256) * cdiv(a.N, 256) >= 192;
-  const int b = big ? 256 : 128;
-  a.tm = (int)cdiv(a.M, b);
-  a.tn = (int)cdiv(a.N, b);
+  constexpr bool dual = MODE >= kHSum;
+  const bool big = big_logits(k, dual, a.M, a.N);
+  a.tm = (int)cdiv(a.M, big ? 256 : 128);
+  a.tn = (int)cdiv(a.N, big && !dual ? 256 : 128);
   const unsigned grid = (unsigned)(a.tm * a.tn);
-#define LOGITS(T, PL)                                                              \
-  do {                                                                             \
-    if constexpr (!dual) {                                                         \
-      if (big) {                                                                   \
-        k_logits<T, 256, 256, 2, 4, MODE, PL><<<grid, 512, 0, st>>>(a);            \
-        break;                                                                     \
-      }                                                                            \
-    }                                                                              \
-    k_logits<T, 128, 128, 2, 2, MODE, PL><<<grid, 256, 0, st>>>(a);                \
-  } while (0)
-  if (k.dtype == TTT_F32) LOGITS(__bf16, 3);
-  else if (k.dtype == TTT_BF16) LOGITS(__bf16, 1);
-  else LOGITS(_Float16, 1);
-#undef LOGITS
-}
-
-// Rows of parts that launch_logits writes for M vocabulary rows (two waves of
-// a tile's vocabulary each).
-int parts_of(bool dual, int M, int N) {
-  const bool big = !dual && cdiv(M, 256) * cdiv(N, 256) >= 192;
-  return (int)cdiv(M, big ? 256 : 128) * 2;
+  if (k.dtype == TTT_F32) {
+    k_logits<float, MODE, false><<<grid, 512, 0, st>>>(a);
+  } else if (k.dtype == TTT_BF16) {
+    if (big) k_logits<__bf16, MODE, true><<<grid, 512, 0, st>>>(a);
+    else k_logits<__bf16, MODE, false><<<grid, 256, 0, st>>>(a);
+  } else {
+    if (big) k_logits<_Float16, MODE, true><<<grid, 512, 0, st>>>(a);
+    else k_logits<_Float16, MODE, false><<<grid, 256, 0, st>>>(a);
+  }
 }
 
 // Makes room in part for the rows of a piece of m vocabulary rows.
-template <int MODE>
-void make_room(const Buffers& b, int N, int m, int* parts, hipStream_t st) {
-  if (*parts + parts_of(MODE == kHSum, m, N) <= b.parts) return;
-  k_merge<MODE><<<(unsigned)cdiv(N, 256), 256, 0, st>>>(b.part, *parts, N);
+template <bool STATS>
+void make_room(const Plan& k, const Buffers& b, int m, int* parts, hipStream_t st) {
+  if (*parts + parts_of(k, !STATS, m, k.N) <= b.parts) return;
+  k_merge<STATS><<<(unsigned)cdiv(k.N, 64), 1024, 0, st>>>(b.part, *parts, k.N);
   *parts = 1;
 }
 
-void launch_finish(const Plan& k, const OutArgs& a, hipStream_t st) {
-  const unsigned grid = (unsigned)cdiv((int64_t)a.N * a.M, 1024);
-  if (k.dtype == TTT_F32) k_finish<float><<<grid, 256, 0, st>>>(a);
-  else if (k.dtype == TTT_BF16) k_finish<__bf16><<<grid, 256, 0, st>>>(a);
-  else k_finish<_Float16><<<grid, 256, 0, st>>>(a);
+template <typename T>
+void launch_product_of(const OutArgs& a, bool nt, bool big, bool fin, hipStream_t st) {
+  const unsigned grid = (unsigned)(a.tm * a.tn * a.split);
+  const unsigned threads = sizeof(T) == 4 || big ? 512 : 256;
+  if constexpr (sizeof(T) == 2) {
+    if (big && nt) k_product<T, true, true><<<grid, threads, 0, st>>>(a);
+    else if (big) k_product<T, false, true><<<grid, threads, 0, st>>>(a);
+  }
+  if (!big && nt) k_product<T, true, false><<<grid, threads, 0, st>>>(a);
+  else if (!big) k_product<T, false, false><<<grid, threads, 0, st>>>(a);
+  if (fin) k_finish<T><<<(unsigned)cdiv((int64_t)a.N * a.M, 1024), 256, 0, st>>>(a);
 }
 
-// One product.  keep: its fp32 parts stay (a later piece adds to them), with
-// the split of the first piece, whose steps are `full`.
-void launch_product(const Plan& k, OutArgs a, float* part, bool keep, int full, bool last, hipStream_t st) {
-  const Spread s = spread_of(a.M, a.N, full);
-  a.tm = s.tm;
-  a.tn = s.tn;
+// One product (nt: its N operand is turned; the M operand always is).  keep:
+// its fp32 parts stay (a later piece adds to them).  s: the spread of a whole
+// piece's product, which the layout has room for; a shorter last piece has the
+// same split (its own could be larger, and its parts past the room).
+void launch_product(const Plan& k, OutArgs a, bool nt, float* part, bool keep, const Spread& s, bool last,
+                    hipStream_t st) {
+  int steps = 0;
+  for (int i = 0; i < a.l.n; ++i) steps += (int)cdiv(a.l.s[i].k, k.f32 ? 32 : 64);
+  a.tm = (int)cdiv(a.M, s.big ? 256 : 128);
+  a.tn = (int)cdiv(a.N, s.big ? 256 : 128);
   a.split = s.split;
-  a.chunk = (int)cdiv(a.l.steps, s.split);
+  a.chunk = (int)cdiv(steps, s.split);
   a.part = keep || s.split > 1 ? part : nullptr;
-  const unsigned grid = (unsigned)(s.tm * s.tn * s.split);
-#define PRODUCT(T, TO)                                                                     \
-  do {                                                                                     \
-    if (s.big) k_product<T, TO, 256, 256, 2, 4><<<grid, 512, 0, st>>>(a);                  \
-    else k_product<T, TO, 128, 128, 2, 2><<<grid, 256, 0, st>>>(a);                        \
-  } while (0)
-  if (k.dtype == TTT_F32) PRODUCT(__bf16, float);
-  else if (k.dtype == TTT_BF16) PRODUCT(__bf16, __bf16);
-  else PRODUCT(_Float16, _Float16);
-#undef PRODUCT
-  if (a.part && last) launch_finish(k, a, st);
+  const bool fin = a.part && last;
+  if (k.dtype == TTT_F32) launch_product_of<float>(a, nt, false, fin, st);
+  else if (k.dtype == TTT_BF16) launch_product_of<__bf16>(a, nt, s.big, fin, st);
+  else launch_product_of<_Float16>(a, nt, s.big, fin, st);
 }
 
 int check(const ttt_lce_problem* p) {
@@ -853,34 +906,103 @@ int finish(const char* what) {
 }
 
 RowArgs row_args(const ttt_lce_problem* p, const Plan& k, const Buffers& b, const int64_t* target,
-                 const float* weight) {
+                 const float* weight, const float* row_stats, const float* grad_loss) {
   RowArgs r;
   memset(&r, 0, sizeof(r));
   r.N = k.N;
   r.V = k.V;
   r.reduction = p->reduction;
-  r.f16 = k.dtype == TTT_F16;
+  r.dtype = k.dtype;
   r.ignore = p->ignore_index;
   r.target = target;
   r.weight = weight;
+  r.stat = const_cast<float*>(row_stats);
+  r.grad_loss = grad_loss;
   r.part = b.part;
   r.at_target = b.at_target;
+  r.h = b.h;
   r.coef = b.coef;
-  r.rowmul = b.rowmul;
+  r.live = b.live;
   r.colmul = b.colmul;
-  r.outmul = b.outmul;
   r.alpha = b.alpha;
   return r;
 }
 
-// Rows v0 .. of w (or b) as an operand over d: packed, or as they are.
-Operand rows_of(const Plan& k, const ttt_rows* w, int v0, int rows, void* packed) {
-  if (k.pack) return {packed, k.dp, (int64_t)rows * k.dp};
-  return {(const char*)w->data + (int64_t)v0 * w->stride * 2, w->stride, 0};
+void launch_factors(const RowArgs& r, hipStream_t st) {
+  k_factors<<<r.dtype == TTT_F32 ? (unsigned)cdiv(r.N, 1024) : 1, 1024, 0, st>>>(r);
 }
-const void* row_at(const Plan& k, const ttt_rows* w, int v0) {
-  return (const char*)w->data + (int64_t)v0 * w->stride * (k.f32 ? 4 : 2);
+
+// Rows v0 .. v0 + rows - 1 of an operand over d: copied, or as they are.
+Operand rows_of(const Plan& k, const ttt_rows* w, int v0, int rows, void* copy, bool fresh, hipStream_t st) {
+  const char* at = (const char*)w->data + (int64_t)v0 * w->stride * k.es;
+  if (!k.pack) return {at, w->stride};
+  if (fresh) launch_copy(at, w->stride, rows, k.d, copy, nullptr, st);
+  return {copy, k.dp};
 }
+
+// X (or A) with zeros in the rows that do not count, where a sum over the rows will
+// meet them (fp32: k_product leaves them out itself).
+Operand live_rows(const Plan& k, const ttt_rows* x, void* copy, bool sums, const float* live, hipStream_t st) {
+  if (k.f32 || (!k.pack && !sums)) return {x->data, x->stride};
+  launch_copy(x->data, x->stride, k.N, k.d, copy, live, st);
+  return {copy, k.dp};
+}
+
+// What the products of a call have in common.
+struct Call {
+  const Plan& k;
+  const Buffers& b;
+  hipStream_t st;
+
+  // z (and u) tiles of vocabulary rows v0 .. v0 + m - 1
+  ZArgs tiles(int v0, int m, const int64_t* target, const float* stat) const {
+    ZArgs a;
+    memset(&a, 0, sizeof(a));
+    a.M = m;
+    a.N = k.N;
+    a.v0 = v0;
+    a.target = target;
+    a.stat = stat;
+    a.h = b.h;
+    a.colmul = b.colmul;
+    return a;
+  }
+  // Operands that are G or H of a piece of m rows
+  Operand piece(const void* g, int m) const { return {g, round8(m)}; }
+
+  // out [N, d] (+)= the list's product over the piece
+  void over_vocab(const SegList& l, const ttt_rows* out, float* out32, bool add, bool keep, bool last) const {
+    OutArgs o;
+    memset(&o, 0, sizeof(o));
+    o.l = l;
+    o.M = k.d;
+    o.N = k.N;
+    if (out) {
+      o.out = out->data;
+      o.ld = out->stride;
+    }
+    o.out32 = out32;
+    o.rows = b.live;
+    o.alpha = b.alpha;
+    o.add = add;
+    launch_product(k, o, false, b.part_x, keep, spread_x(k, l.n, keep), last, st);
+  }
+  // out rows v0 .. [m, d] = the list's product over the tokens
+  void over_rows(const SegList& l, const ttt_rows* out, int v0, int m) const {
+    OutArgs o;
+    memset(&o, 0, sizeof(o));
+    o.l = l;
+    o.M = k.d;
+    o.N = m;
+    o.out = (char*)out->data + (int64_t)v0 * out->stride * k.es;
+    o.ld = out->stride;
+    o.live = k.f32 ? b.live : nullptr;
+    o.alpha = b.alpha;
+    launch_product(k, o, true, b.part_w, false, spread_w(k, l.n), true, st);
+  }
+};
+
+bool given(const ttt_rows* r) { return r && r->data; }
 
 }  // namespace
 }  // namespace ttt
@@ -911,39 +1033,31 @@ int ttt_lce_fwd(const ttt_lce_problem* p, const ttt_rows* x, const ttt_rows* w, 
   Buffers b;
   TRY(workspace(k, ws, ws_bytes, "ttt_lce_fwd", &b));
   const hipStream_t st = (hipStream_t)stream;
-  if (k.pack) launch_pack(k, x->data, x->stride, k.N, k.d, b.xr, nullptr, nullptr, st);
-  const Operand xo = rows_of(k, x, 0, k.N, b.xr);
+  const Call call{k, b, st};
+  const Operand xo = rows_of(k, x, 0, k.N, b.xr, true, st);
   int parts = 0;
   for (int v0 = 0; v0 < k.V; v0 += k.vc) {
     const int m = k.V - v0 < k.vc ? k.V - v0 : k.vc;
-    if (k.pack) launch_pack(k, row_at(k, w, v0), w->stride, m, k.d, b.wr, nullptr, nullptr, st);
-    const Operand wo = rows_of(k, w, v0, m, b.wr);
-    ZArgs a;
-    memset(&a, 0, sizeof(a));
-    add_product(&a.z, k, wo.p, wo.ld, wo.plane, xo.p, xo.ld, xo.plane, k.dp);
-    a.M = m;
-    a.N = k.N;
-    a.v0 = v0;
-    a.target = target;
-    make_room<kStats>(b, k.N, m, &parts, st);
+    ZArgs a = call.tiles(v0, m, target, nullptr);
+    add_product(&a.z, rows_of(k, w, v0, m, b.wr, true, st), xo, k.f32 ? k.d : k.dp);
+    make_room<true>(k, b, m, &parts, st);
     a.part = b.part + (int64_t)parts * k.N;
     a.at_target = b.at_target;
     launch_logits<kStats>(k, a, st);
-    parts += parts_of(false, m, k.N);
+    parts += parts_of(k, false, m, k.N);
   }
-  RowArgs r = row_args(p, k, b, target, row_weight);
+  RowArgs r = row_args(p, k, b, target, row_weight, row_stats, nullptr);
   r.parts = parts;
-  r.stat = row_stats;
   r.row = p->reduction == TTT_REDUCE_NONE ? loss : b.row;
   r.out = loss;
-  k_join_loss<<<(unsigned)cdiv(k.N, 256), 256, 0, st>>>(r);
+  k_join_loss<<<(unsigned)cdiv(k.N, 64), 1024, 0, st>>>(r);
   k_reduce_loss<<<1, 1024, 0, st>>>(r);
   return finish("ttt_lce_fwd");
 }
 
 int ttt_lce_bwd(const ttt_lce_problem* p, const ttt_rows* x, const ttt_rows* w, const int64_t* target,
                 const float* row_weight, const float* row_stats, const float* grad_loss, const ttt_rows* dx,
-                const ttt_rows* dw, void* ws, int64_t ws_bytes, void* stream) {
+                const ttt_rows* dw, float* dx32, void* ws, int64_t ws_bytes, void* stream) {
   TRY(check(p));
   TRY(take(p, x, "hidden", true, true));
   TRY(take(p, w, "weight", true, true));
@@ -951,68 +1065,41 @@ int ttt_lce_bwd(const ttt_lce_problem* p, const ttt_rows* x, const ttt_rows* w, 
   TRY(take(p, dw, "dw", false, false));
   if (!target || !row_stats || !grad_loss)
     return ops_fail(TTT_ERR_INVALID_ARGUMENT, "linear cross entropy: target, row_stats and grad_loss are needed");
-  const bool want_x = dx && dx->data, want_w = dw && dw->data;
+  const bool want_x = given(dx), want_w = given(dw);
+  if (dx32 && !want_x) return ops_fail(TTT_ERR_INVALID_ARGUMENT, "ttt_lce_bwd: dx32 without dx");
   if (!want_x && !want_w) return TTT_OK;
   const Plan k = plan_of(p, TTT_LCE_BWD);
   Buffers b;
   TRY(workspace(k, ws, ws_bytes, "ttt_lce_bwd", &b));
   const hipStream_t st = (hipStream_t)stream;
-  RowArgs r = row_args(p, k, b, target, row_weight);
-  r.stat = const_cast<float*>(row_stats);
-  r.grad_loss = grad_loss;
-  k_factors<<<r.f16 ? 1 : (unsigned)cdiv(k.N, 1024), 1024, 0, st>>>(r);
-  launch_pack(k, x->data, x->stride, k.N, k.d, k.pack ? b.xr : nullptr, want_w ? b.xt : nullptr, b.coef, st);
-  const Operand xo = rows_of(k, x, 0, k.N, b.xr);
-  int full = 0;
+  const Call call{k, b, st};
+  launch_factors(row_args(p, k, b, target, row_weight, row_stats, grad_loss), st);
+  const Operand xo = live_rows(k, x, b.xr, want_w, b.live, st);
   for (int v0 = 0; v0 < k.V; v0 += k.vc) {
-    const int m = k.V - v0 < k.vc ? k.V - v0 : k.vc, mp = round8(m);
-    launch_pack(k, row_at(k, w, v0), w->stride, m, k.d, k.pack ? b.wr : nullptr, want_x ? b.wt : nullptr, nullptr, st);
-    const Operand wo = rows_of(k, w, v0, m, b.wr);
-    ZArgs a;
-    memset(&a, 0, sizeof(a));
-    add_product(&a.z, k, wo.p, wo.ld, wo.plane, xo.p, xo.ld, xo.plane, k.dp);
-    a.M = m;
-    a.N = k.N;
-    a.v0 = v0;
-    a.target = target;
-    a.stat = row_stats;
-    a.rowmul = b.rowmul;
-    a.colmul = b.colmul;
-    a.grow = want_x ? b.grow : nullptr;
-    a.gcol = want_w ? b.gcol : nullptr;
+    const int m = k.V - v0 < k.vc ? k.V - v0 : k.vc;
+    const Operand wo = rows_of(k, w, v0, m, b.wr, true, st), go = call.piece(b.g, m);
+    ZArgs a = call.tiles(v0, m, target, row_stats);
+    add_product(&a.z, wo, xo, k.f32 ? k.d : k.dp);
+    a.g = b.g;
     launch_logits<kGrad>(k, a, st);
     if (want_x) {
-      OutArgs o;
-      memset(&o, 0, sizeof(o));
-      add_product(&o.l, k, b.wt, mp, (int64_t)k.d * mp, b.grow, mp, (int64_t)k.N * mp, mp);
-      o.M = k.d;
-      o.N = k.N;
-      o.out = dx->data;
-      o.ld = dx->stride;
-      o.mul = b.outmul;
-      o.add = v0 > 0;
-      if (v0 == 0) full = o.l.steps;
-      launch_product(k, o, b.part_x, k.pieces > 1, full, v0 + m >= k.V, st);
+      SegList l{};
+      add_product(&l, wo, go, m);
+      call.over_vocab(l, dx, dx32, v0 > 0, k.pieces > 1, v0 + m >= k.V);
     }
     if (want_w) {
-      OutArgs o;
-      memset(&o, 0, sizeof(o));
-      add_product(&o.l, k, b.xt, k.Np, (int64_t)k.d * k.Np, b.gcol, k.Np, (int64_t)m * k.Np, k.Np);
-      o.M = k.d;
-      o.N = m;
-      o.out = (char*)dw->data + (int64_t)v0 * dw->stride * (k.f32 ? 4 : 2);
-      o.ld = dw->stride;
-      o.alpha = b.alpha;
-      launch_product(k, o, b.part_w, false, o.l.steps, true, st);
+      SegList l{};
+      add_product(&l, xo, go, k.N);
+      call.over_rows(l, dw, v0, m);
     }
   }
   return finish("ttt_lce_bwd");
 }
 
 int ttt_lce_gg(const ttt_lce_problem* p, const ttt_rows* x, const ttt_rows* w, const int64_t* target,
-               const float* row_weight, const float* row_stats, const float* grad_loss, const ttt_rows* ca,
-               const ttt_rows* cb, const ttt_rows* gx, const ttt_rows* gw, float* ggrad_loss, void* ws,
-               int64_t ws_bytes, void* stream) {
+               const float* row_weight, const float* row_stats, const float* grad_loss, const float* dx32,
+               const ttt_rows* ca, const ttt_rows* cb, const ttt_rows* gx, const ttt_rows* gw, float* ggrad_loss,
+               void* ws, int64_t ws_bytes, void* stream) {
   TRY(check(p));
   TRY(take(p, x, "hidden", true, true));
   TRY(take(p, w, "weight", true, true));
@@ -1022,8 +1109,7 @@ int ttt_lce_gg(const ttt_lce_problem* p, const ttt_rows* x, const ttt_rows* w, c
   TRY(take(p, gw, "gw", false, false));
   if (!target || !row_stats || !grad_loss)
     return ops_fail(TTT_ERR_INVALID_ARGUMENT, "linear cross entropy: target, row_stats and grad_loss are needed");
-  const bool has_a = ca && ca->data, has_b = cb && cb->data;
-  const bool want_x = gx && gx->data, want_w = gw && gw->data;
+  const bool has_a = given(ca), has_b = given(cb), want_x = given(gx), want_w = given(gw);
   if (!has_a && !has_b)
     return ops_fail(TTT_ERR_INVALID_ARGUMENT, "ttt_lce_gg: a cotangent of dx or of dw is needed");
   if (!want_x && !want_w && !ggrad_loss) return TTT_OK;
@@ -1031,98 +1117,118 @@ int ttt_lce_gg(const ttt_lce_problem* p, const ttt_rows* x, const ttt_rows* w, c
   Buffers b;
   TRY(workspace(k, ws, ws_bytes, "ttt_lce_gg", &b));
   const hipStream_t st = (hipStream_t)stream;
-  RowArgs r = row_args(p, k, b, target, row_weight);
-  r.stat = const_cast<float*>(row_stats);
-  r.grad_loss = grad_loss;
-  // c before the transposes (rows of factor 0 are left out of them); fp16's scales follow the first pass
-  r.f16 = 0;
-  k_factors<<<(unsigned)cdiv(k.N, 1024), 1024, 0, st>>>(r);
-  launch_pack(k, x->data, x->stride, k.N, k.d, k.pack ? b.xr : nullptr, want_w ? b.xt : nullptr, b.coef, st);
-  if (has_a)
-    launch_pack(k, ca->data, ca->stride, k.N, k.d, k.pack ? b.ar : nullptr, want_w ? b.at : nullptr, b.coef, st);
-  const Operand xo = rows_of(k, x, 0, k.N, b.xr);
-  Operand ao{nullptr, 0, 0};
-  if (has_a) ao = rows_of(k, ca, 0, k.N, b.ar);
-  const bool second = want_x || want_w;
-  int parts = 0, full = 0;
-  for (int pass = 0; pass < (second ? 2 : 1); ++pass) {
-    for (int v0 = 0; v0 < k.V; v0 += k.vc) {
-      const int m = k.V - v0 < k.vc ? k.V - v0 : k.vc, mp = round8(m);
-      const bool turned = pass == 1 && want_x;
-      const bool fresh = pass == 0 || k.pieces > 1;  // one piece: the rows packed for the first pass are there
-      launch_pack(k, row_at(k, w, v0), w->stride, m, k.d, k.pack && fresh ? b.wr : nullptr, turned ? b.wt : nullptr,
-                  nullptr, st);
-      if (has_b)
-        launch_pack(k, row_at(k, cb, v0), cb->stride, m, k.d, k.pack && fresh ? b.br : nullptr,
-                    turned ? b.bt : nullptr, nullptr, st);
-      const Operand wo = rows_of(k, w, v0, m, b.wr);
-      ZArgs a;
-      memset(&a, 0, sizeof(a));
-      add_product(&a.z, k, wo.p, wo.ld, wo.plane, xo.p, xo.ld, xo.plane, k.dp);
-      if (has_a) add_product(&a.u, k, wo.p, wo.ld, wo.plane, ao.p, ao.ld, ao.plane, k.dp);
-      if (has_b) {
-        const Operand bo = rows_of(k, cb, v0, m, b.br);
-        add_product(&a.u, k, bo.p, bo.ld, bo.plane, xo.p, xo.ld, xo.plane, k.dp);
-      }
-      a.M = m;
-      a.N = k.N;
-      a.v0 = v0;
-      a.target = target;
-      a.stat = row_stats;
-      if (pass == 0) {
-        make_room<kHSum>(b, k.N, m, &parts, st);
-        a.part = b.part + (int64_t)parts * k.N;
-        a.at_target = b.at_target;
-        launch_logits<kHSum>(k, a, st);
-        parts += parts_of(true, m, k.N);
-        continue;
-      }
-      a.h = b.h;
-      a.rowmul = b.rowmul;
-      a.colmul = b.colmul;
-      a.hrow = want_x ? b.hrow : nullptr;
-      a.hcol = want_w ? b.hcol : nullptr;
-      a.grow = want_x && has_b ? b.grow : nullptr;
-      a.gcol = want_w && has_a ? b.gcol : nullptr;
-      launch_logits<kHGrad>(k, a, st);
-      if (want_x) {
-        OutArgs o;
-        memset(&o, 0, sizeof(o));
-        add_product(&o.l, k, b.wt, mp, (int64_t)k.d * mp, b.hrow, mp, (int64_t)k.N * mp, mp);
-        if (has_b) add_product(&o.l, k, b.bt, mp, (int64_t)k.d * mp, b.grow, mp, (int64_t)k.N * mp, mp);
-        o.M = k.d;
-        o.N = k.N;
-        o.out = gx->data;
-        o.ld = gx->stride;
-        o.mul = b.outmul;
-        o.add = v0 > 0;
-        if (v0 == 0) full = o.l.steps;
-      launch_product(k, o, b.part_x, k.pieces > 1, full, v0 + m >= k.V, st);
-      }
-      if (want_w) {
-        OutArgs o;
-        memset(&o, 0, sizeof(o));
-        add_product(&o.l, k, b.xt, k.Np, (int64_t)k.d * k.Np, b.hcol, k.Np, (int64_t)m * k.Np, k.Np);
-        if (has_a) add_product(&o.l, k, b.at, k.Np, (int64_t)k.d * k.Np, b.gcol, k.Np, (int64_t)m * k.Np, k.Np);
-        o.M = k.d;
-        o.N = m;
-        o.out = (char*)gw->data + (int64_t)v0 * gw->stride * (k.f32 ? 4 : 2);
-        o.ld = gw->stride;
-        o.alpha = b.alpha;
-        launch_product(k, o, b.part_w, false, o.l.steps, true, st);
-      }
+  const Call call{k, b, st};
+  RowArgs r = row_args(p, k, b, target, row_weight, row_stats, grad_loss);
+  if (k.dtype == TTT_F16) {
+    const auto norms = [&](const ttt_rows* t, int rows, float* out) {
+      k_norms<_Float16><<<(unsigned)cdiv(rows, 4), 256, 0, st>>>((const _Float16*)t->data, t->stride, rows, k.d, out);
+      return out;
+    };
+    if (has_a) {
+      r.na = norms(ca, k.N, b.na);
+      r.nw = norms(w, k.V, b.nw);
     }
-    if (pass == 0) {
-      r.parts = parts;
-      r.h = b.h;
-      r.umax = k.dtype == TTT_F16 ? b.umax : nullptr;
-      r.row = ggrad_loss ? (p->reduction == TTT_REDUCE_NONE ? ggrad_loss : b.row) : nullptr;
-      k_join_h<<<(unsigned)cdiv(k.N, 256), 256, 0, st>>>(r);
-      if (ggrad_loss && p->reduction != TTT_REDUCE_NONE) k_sum<<<1, 1024, 0, st>>>(b.row, k.N, ggrad_loss);
-      if (second && k.dtype == TTT_F16) {
-        r.f16 = 1;
-        k_factors<<<1, 1024, 0, st>>>(r);
+    if (has_b) {
+      r.nx = norms(x, k.N, b.nx);
+      r.nb = norms(cb, k.V, b.nb);
+    }
+  }
+  launch_factors(r, st);
+  const Operand xo = live_rows(k, x, b.xr, want_w, b.live, st);
+  Operand ao{nullptr, 0};
+  if (has_a) ao = live_rows(k, ca, b.ar, want_w, b.live, st);
+  const int kd = k.f32 ? k.d : k.dp;
+  const bool second = want_x || want_w;
+  // h from dX and G B, or from its tiles
+  const bool sums = ggrad_loss || (has_a && !dx32);
+  const bool one = k.pieces == 1;  // a piece's copies and G last from the first walk to the second
+  const auto zu = [&](int v0, int m, bool fresh, bool u) {
+    ZArgs a = call.tiles(v0, m, target, row_stats);
+    const Operand wo = rows_of(k, w, v0, m, b.wr, fresh, st);
+    add_product(&a.z, wo, xo, kd);
+    if (u && has_a) add_product(&a.u, wo, ao, kd);
+    if (u && has_b) add_product(&a.u, rows_of(k, cb, v0, m, b.br, fresh, st), xo, kd);
+    return a;
+  };
+  bool walked = false;
+  if (sums) {
+    int parts = 0;
+    for (int v0 = 0; v0 < k.V; v0 += k.vc) {
+      const int m = k.V - v0 < k.vc ? k.V - v0 : k.vc;
+      ZArgs a = zu(v0, m, true, true);
+      make_room<false>(k, b, m, &parts, st);
+      a.part = b.part + (int64_t)parts * k.N;
+      a.at_target = b.at_target;
+      launch_logits<kHSum>(k, a, st);
+      parts += parts_of(k, true, m, k.N);
+    }
+    walked = true;
+    r.parts = parts;
+    r.row = ggrad_loss ? (p->reduction == TTT_REDUCE_NONE ? ggrad_loss : b.row) : nullptr;
+    k_join_h<<<(unsigned)cdiv(k.N, 64), 1024, 0, st>>>(r);
+    if (ggrad_loss && p->reduction != TTT_REDUCE_NONE) k_sum<<<1, 1024, 0, st>>>(b.row, k.N, ggrad_loss);
+  } else {
+    HArgs h;
+    memset(&h, 0, sizeof(h));
+    if (has_b) {  // G B to the parts, where H W is added later
+      for (int v0 = 0; v0 < k.V; v0 += k.vc) {
+        const int m = k.V - v0 < k.vc ? k.V - v0 : k.vc;
+        ZArgs a = zu(v0, m, true, false);
+        a.g = b.g;
+        launch_logits<kGrad>(k, a, st);
+        SegList l{};
+        add_product(&l, rows_of(k, cb, v0, m, b.br, true, st), call.piece(b.g, m), m);
+        call.over_vocab(l, nullptr, nullptr, v0 > 0, true, false);
       }
+      walked = true;
+      h.gb = b.part_x;
+      h.split = spread_x(k, 1, true).split;
+      h.b = cb->data;
+      h.ldb = cb->stride;
+    }
+    if (has_a) {
+      h.a = ca->data;
+      h.lda = ca->stride;
+      h.dx32 = dx32;
+    }
+    h.N = k.N;
+    h.V = k.V;
+    h.d = k.d;
+    h.target = target;
+    h.coef = b.coef;
+    h.alpha = b.alpha;
+    h.x = x->data;
+    h.ldx = x->stride;
+    h.w = w->data;
+    h.ldw = w->stride;
+    h.h = b.h;
+    const unsigned grid = (unsigned)cdiv(k.N, 4);
+    if (k.dtype == TTT_F32) k_row_h<float><<<grid, 256, 0, st>>>(h);
+    else if (k.dtype == TTT_BF16) k_row_h<__bf16><<<grid, 256, 0, st>>>(h);
+    else k_row_h<_Float16><<<grid, 256, 0, st>>>(h);
+  }
+  if (!second) return finish("ttt_lce_gg");
+  const bool kept = !sums && has_b;  // G B waits in the parts
+  for (int v0 = 0; v0 < k.V; v0 += k.vc) {
+    const int m = k.V - v0 < k.vc ? k.V - v0 : k.vc;
+    const bool fresh = !(walked && one);
+    ZArgs a = zu(v0, m, fresh, true);
+    const bool need_g = (want_x && has_b && sums) || (want_w && has_a);
+    a.hh = b.hh;
+    a.g = need_g && !(kept && one) ? b.g : nullptr;
+    launch_logits<kHGrad>(k, a, st);
+    const Operand go = call.piece(b.g, m), ho = call.piece(b.hh, m);
+    if (want_x) {
+      SegList l{};
+      add_product(&l, rows_of(k, w, v0, m, b.wr, false, st), ho, m);
+      if (has_b && sums) add_product(&l, rows_of(k, cb, v0, m, b.br, false, st), go, m);
+      call.over_vocab(l, gx, nullptr, v0 > 0 || kept, k.pieces > 1 || kept, v0 + m >= k.V);
+    }
+    if (want_w) {
+      SegList l{};
+      add_product(&l, xo, ho, k.N);
+      if (has_a) add_product(&l, ao, go, k.N);
+      call.over_rows(l, gw, v0, m);
     }
   }
   return finish("ttt_lce_gg");

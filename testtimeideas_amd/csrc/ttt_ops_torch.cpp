@@ -330,18 +330,19 @@ std::vector<Tensor> lce_fwd(const Tensor& x_, const Tensor& w_, const Tensor& ta
   return {loss, stats};
 }
 
-// dx, dw: those asked for.
+// dx, dw: those asked for; and dx32 with `keep`.
 std::vector<Tensor> lce_bwd(const Tensor& g, const Tensor& x_, const Tensor& w_, const Tensor& target,
                             const Tensor& mask, const Tensor& stats, int64_t reduction, int64_t ignore, bool nx,
-                            bool nw) {
+                            bool nw, bool keep) {
   const Launch on(x_);
   const Tensor x = lce_rows(x_), w = lce_rows(w_);
-  Tensor dx, dw;
+  Tensor dx, dw, dx32;
   if (nx) dx = at::empty(x_.sizes(), x_.options());
+  if (nx && keep) dx32 = at::empty(x_.sizes(), x_.options().dtype(at::kFloat));
   if (nw) dw = at::empty(w_.sizes(), w_.options());
   if (x.size(0) == 0) {
     if (nw) dw.zero_();
-    return {dx, dw};
+    return {dx, dw, dx32};
   }
   const ttt_lce_problem p = lce_problem(x, w, reduction, ignore);
   int64_t nb;
@@ -351,10 +352,10 @@ std::vector<Tensor> lce_bwd(const Tensor& g, const Tensor& x_, const Tensor& w_,
   rdx.data = ptr(dx);
   rdw.data = ptr(dw);
   rdx.stride = rdw.stride = x.size(1);
-  check(ttt_lce_bwd(&p, &rx, &rw, target.data_ptr<int64_t>(), fptr(mask), fptr(stats), fptr(g), &rdx, &rdw, ptr(ws),
-                    nb, on.stream()),
+  check(ttt_lce_bwd(&p, &rx, &rw, target.data_ptr<int64_t>(), fptr(mask), fptr(stats), fptr(g), &rdx, &rdw,
+                    fptr(dx32), ptr(ws), nb, on.stream()),
         "ttt_lce_bwd");
-  return {dx, dw};
+  return {dx, dw, dx32};
 }
 
 struct LceBwd : public torch::autograd::Function<LceBwd> {
@@ -362,16 +363,16 @@ struct LceBwd : public torch::autograd::Function<LceBwd> {
                                const Tensor& target, const OptTensor& mask_, const Tensor& stats, int64_t reduction,
                                int64_t ignore, bool nx, bool nw) {
     const Tensor mask = tensor_of(mask_);
-    const std::vector<Tensor> r = lce_bwd(g, x, w, target, mask, stats, reduction, ignore, nx, nw);
-    ctx->save_for_backward({g, x, w, target, mask, stats});
+    const std::vector<Tensor> r = lce_bwd(g, x, w, target, mask, stats, reduction, ignore, nx, nw, true);
+    ctx->save_for_backward({g, x, w, target, mask, stats, r[2]});
     ctx->saved_data["reduction"] = reduction;
     ctx->saved_data["ignore"] = ignore;
     ctx->saved_data["nx"] = nx;
     ctx->saved_data["nw"] = nw;
     ctx->set_materialize_grads(false);
     variable_list out;
-    for (const Tensor& t : r)
-      if (t.defined()) out.push_back(t);
+    if (nx) out.push_back(r[0]);
+    if (nw) out.push_back(r[1]);
     return out;
   }
 
@@ -404,8 +405,8 @@ struct LceBwd : public torch::autograd::Function<LceBwd> {
         rgx.data = ptr(gx);
         rgw.data = ptr(gw);
         rgx.stride = rgw.stride = x.size(1);
-        check(ttt_lce_gg(&p, &rx, &rw, s[3].data_ptr<int64_t>(), fptr(s[4]), fptr(s[5]), fptr(s[0]), &ra, &rb, &rgx,
-                         &rgw, fptr(gg), ptr(ws), nb, on.stream()),
+        check(ttt_lce_gg(&p, &rx, &rw, s[3].data_ptr<int64_t>(), fptr(s[4]), fptr(s[5]), fptr(s[0]), fptr(s[6]), &ra,
+                         &rb, &rgx, &rgw, fptr(gg), ptr(ws), nb, on.stream()),
               "ttt_lce_gg");
       }
       out[0] = gg;
@@ -442,8 +443,9 @@ struct Lce : public torch::autograd::Function<Lce> {
     if (at::GradMode::is_enabled()) {
       r = LceBwd::apply(go, s[0], s[1], s[2], opt(s[3]), s[4], reduction, ignore, nx, nw);
     } else {
-      for (const Tensor& t : lce_bwd(go, s[0], s[1], s[2], s[3], s[4], reduction, ignore, nx, nw))
-        if (t.defined()) r.push_back(t);
+      const std::vector<Tensor> d = lce_bwd(go, s[0], s[1], s[2], s[3], s[4], reduction, ignore, nx, nw, false);
+      if (nx) r.push_back(d[0]);
+      if (nw) r.push_back(d[1]);
     }
     size_t n = 0;
     if (nx) out[0] = r[n++];
