@@ -134,7 +134,7 @@ def test_lce_refusals():
 def test_lce_workspace_does_not_grow_with_the_logits():
     """Past a piece's size, the workspace is that of a piece."""
     size = lambda v, e: _c().ttt_lce_workspace_size(ctypes.byref(Lce(1, 2, 8192, 512, v, -100)), e)  # noqa: E731
-    assert all(size(1 << 22, e) <= 1.1 * size(1 << 17, e) for e in (0, 1, 2))
+    assert all(size(1 << 22, e) <= 1.1 * size(1 << 18, e) for e in (0, 1, 2))
     assert size(1 << 22, 1) < 8192 * (1 << 22) * 2 / 64
     assert size(0, 1) == -1 and size(64, 3) == -1
 

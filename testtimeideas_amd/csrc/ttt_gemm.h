@@ -103,19 +103,27 @@ struct Loader {
   static __device__ __forceinline__ int swz(int k) {
     return ((k & 1) << 1) | (((k >> 1) & 1) << 2) | (((k >> 3) & 1) << 3);
   }
-  static __device__ __forceinline__ int row_of(int q, int wave) {
-    return (1024 * (wave + NW * q) + 16 * (int)(threadIdx.x & 63)) / kRowBytes;
+  // Row and chunk that instruction q fetches in this lane.  They are needed
+  // where a segment begins or ends only: `lane` is made opaque there, or they
+  // would be kept in registers all along.
+  static __device__ __forceinline__ int fresh_lane() {
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    return lane;
   }
-  static __device__ __forceinline__ int chunk_of(int row) {
-    const int slot = (int)(threadIdx.x & 63) % kChunks;
-    return slot ^ (TURNED ? swz(row) : row & 7);
+  static __device__ __forceinline__ int row_of(int q, int wave, int lane) {
+    return (1024 * (wave + NW * q) + 16 * lane) / kRowBytes;
+  }
+  static __device__ __forceinline__ int chunk_of(int row, int lane) {
+    return lane % kChunks ^ (TURNED ? swz(row) : row & 7);
   }
   // valid: rows (turned: columns) of the tile that exist
   __device__ __forceinline__ void enter(int valid, int64_t ld, int wave) {
     step = TURNED ? 128 * ld : 128;
+    const int lane = fresh_lane();
 #pragma unroll
     for (int q = 0; q < kPerWave; ++q) {
-      const int r = row_of(q, wave), ch = chunk_of(r);
+      const int r = row_of(q, wave, lane), ch = chunk_of(r, lane);
       const bool in = TURNED ? 8 * ch < valid : r < valid;
       off[q] = in ? (uint32_t)r * (uint32_t)(ld * 2) + 16u * (uint32_t)ch : kBufRange;
     }
@@ -131,10 +139,11 @@ struct Loader {
         __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void_t*)(lds + 1024 * (wave + NW * q)), 16, (int)off[q], 0, 0,
                                                  0);
     } else {
+      const int lane = fresh_lane();
 #pragma unroll
       for (int q = 0; q < kPerWave; ++q) {
-        const int row = row_of(q, wave);
-        const bool in = TURNED ? row < left : 8 * chunk_of(row) < left;
+        const int row = row_of(q, wave, lane);
+        const bool in = TURNED ? row < left : 8 * chunk_of(row, lane) < left;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void_t*)(lds + 1024 * (wave + NW * q)), 16,
                                                  in ? (int)off[q] : kBufPast, 0, 0, 0);
       }
@@ -163,12 +172,14 @@ struct TileProduct : TileBase<BM_, BN_, WM_, WN_, 64> {
   Loader<BM, NW, MT> lm;
   Loader<BN, NW, NT> ln;
   const char *bm, *bn;
+  int kseg;  // the segment's k
 
   __device__ __forceinline__ TileProduct(int m0, int n0, int M, int N) : B(m0, n0, M, N) {}
 
   __device__ __forceinline__ void enter(const SegList& l) {
     const Seg& s = l.s[this->seg];
     const int64_t k0 = this->k0;
+    kseg = s.k;
     bm = (const char*)s.m + (MT ? k0 * s.ldm + this->m0 : this->m0 * s.ldm + k0) * 2;
     bn = (const char*)s.n + (NT ? k0 * s.ldn + this->n0 : this->n0 * s.ldn + k0) * 2;
     lm.enter(this->mrows, s.ldm, this->wave);
@@ -176,7 +187,7 @@ struct TileProduct : TileBase<BM_, BN_, WM_, WN_, 64> {
   }
   // Issue the loads of the current step and move to the next.
   __device__ __forceinline__ void issue(const SegList& l, char* sm, char* sn, bool last) {
-    const int left = l.s[this->seg].k - this->k0;
+    const int left = kseg - this->k0;
     lm.issue(sm, bm, left, this->wave);
     ln.issue(sn, bn, left, this->wave);
     this->k0 += 64;
@@ -189,18 +200,24 @@ struct TileProduct : TileBase<BM_, BN_, WM_, WN_, 64> {
     }
   }
 
-  // Row fragment of rows r0 .. r0 + 15: eight k of row r0 + c, from 32 kk + 8 g.
+  // This lane's byte offset of a fragment's eight k (of row c, from 8 g) in the
+  // tile of an operand whose fragments start at row r0 of R.  Fragment i is at
+  // the offset + 2048 i, turned: offset ^ 32 i; 32 k on: ^ 64, turned: + 64 R.
   template <int R, bool TURNED>
-  static __device__ __forceinline__ frag read(const char* s, int r0, int kk) {
+  static __device__ __forceinline__ int lane_offset(int r0) {
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    if constexpr (!TURNED) return (r0 + c) * 128 + 16 * (g ^ (c & 7));
+    const int k = 8 * g + (c >> 2);  // k + 4 and k + 32 have the same permutation
+    return k * (R * 2) + 16 * (((r0 >> 3) + ((c & 3) >> 1)) ^ Loader<R, NW, true>::swz(k)) + 8 * (c & 1);
+  }
+  template <int R, bool TURNED>
+  static __device__ __forceinline__ frag read(const char* s, int off, int i, int kk) {
     if constexpr (!TURNED) {
-      return *(const frag*)(s + (r0 + c) * 128 + 16 * ((4 * kk + g) ^ (c & 7)));
+      return *(const frag*)(s + (off ^ (64 * kk)) + 2048 * i);
     } else {
-      const int k = 32 * kk + 8 * g + (c >> 2);  // k + 4 has the same permutation
-      const int col = r0 + 4 * (c & 3);
-      const char* a = s + k * (R * 2) + 16 * ((col >> 3) ^ Loader<R, NW, true>::swz(k)) + 2 * (col & 7);
+      const char* a = s + (off ^ (32 * i)) + kk * 64 * R;
       const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(a));
-      const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(a + 4 * R * 2));
+      const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(a + 8 * R));
       const i16x4 both[2] = {lo, hi};
       frag f;
       __builtin_memcpy(&f, both, 16);
@@ -208,19 +225,74 @@ struct TileProduct : TileBase<BM_, BN_, WM_, WN_, 64> {
     }
   }
 
-  __device__ __forceinline__ void multiply(f32x4 (&acc)[MI][NI], const char* sm, const char* sn) const {
+  // A step is four quarters: 32 k of one half of the M fragments.  The reads
+  // of a quarter's fragments are issued among the products of the quarter
+  // before, across the barrier too, so that neither unit waits for the other.
+  static constexpr int MH = MI / 2;
+  struct Frags {
+    frag n[2][NI];  // of k 0-31 and 32-63
+    frag m[2][MH];  // of the even and odd quarters
+    int om, on;     // lane_offset of the operands
+  };
+  template <int Q>
+  __device__ __forceinline__ void read_quarter(Frags& f, const char* sm, const char* sn) const {
+    constexpr int kk = Q >> 1, h = Q & 1;
+    if constexpr (h == 0)
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      frag fm[MI], fn[NI];
+      for (int i = 0; i < NI; ++i) f.n[kk][i] = read<BN, NT>(sn, f.on, i, kk);
 #pragma unroll
-      for (int i = 0; i < MI; ++i) fm[i] = read<BM, MT>(sm, (this->wm * MI + i) * 16, kk);
+    for (int i = 0; i < MH; ++i) f.m[h][i] = read<BM, MT>(sm, f.om, h * MH + i, kk);
+  }
+  template <int Q>
+  static __device__ __forceinline__ void multiply(f32x4 (&acc)[MI][NI], const Frags& f) {
+    constexpr int kk = Q >> 1, h = Q & 1;
 #pragma unroll
-      for (int i = 0; i < NI; ++i) fn[i] = read<BN, NT>(sn, (this->wn * NI + i) * 16, kk);
+    for (int i = 0; i < MH; ++i)
 #pragma unroll
-      for (int i = 0; i < MI; ++i)
+      for (int j = 0; j < NI; ++j) acc[h * MH + i][j] = Elem<T>::mma(acc[h * MH + i][j], f.m[h][i], f.n[kk][j]);
+  }
+  // The order of the reads of quarter Q (two for a turned fragment) and the
+  // products of the quarter before.
+  template <int Q>
+  static __device__ __forceinline__ void interleave() {
+    constexpr int kReads = MH * (MT ? 2 : 1) + (Q & 1 ? 0 : NI * (NT ? 2 : 1)), kProducts = MH * NI;
+    constexpr int kPer = kProducts / kReads < 1 ? 1 : kProducts / kReads;
 #pragma unroll
-        for (int j = 0; j < NI; ++j) acc[i][j] = Elem<T>::mma(acc[i][j], fm[i], fn[j]);
+    for (int i = 0; i < kReads; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, kPer, 0);
     }
+    __builtin_amdgcn_sched_group_barrier(0x008, kProducts, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+
+  // One step of run(): its tile is in (sm, sn) once the loads are waited for,
+  // the next one's go to (om, on).
+  template <bool FIRST>
+  __device__ __forceinline__ void step(f32x4 (&acc)[MI][NI], Frags& f, const SegList& l, const char* sm, const char* sn,
+                                       char* om, char* on, int left) {
+    dma_wait();
+    __syncthreads();
+    if (left > 1) issue(l, om, on, left <= 2);
+    // the turned reads' addresses are formed here, in every step: kept across
+    // the loop, one for each fragment and buffer, they do not fit the registers
+    if constexpr (MT) asm volatile("" : "+v"(f.om));
+    if constexpr (NT) asm volatile("" : "+v"(f.on));
+    __builtin_amdgcn_sched_barrier(0);
+    read_quarter<0>(f, sm, sn);
+    if constexpr (!FIRST) {
+      multiply<3>(acc, f);
+      interleave<0>();
+    }
+    read_quarter<1>(f, sm, sn);
+    multiply<0>(acc, f);
+    interleave<1>();
+    read_quarter<2>(f, sm, sn);
+    multiply<1>(acc, f);
+    interleave<2>();
+    read_quarter<3>(f, sm, sn);
+    multiply<2>(acc, f);
+    interleave<3>();
   }
 
   // acc += the steps lo .. hi - 1 of the list.  Ends with every wave past its
@@ -230,17 +302,17 @@ struct TileProduct : TileBase<BM_, BN_, WM_, WN_, 64> {
     this->seek(l, lo);
     enter(l);
     issue(l, s.m0, s.n0, lo + 1 >= hi);
-    for (int t = lo; t < hi; t += 2) {
-      dma_wait();
-      __syncthreads();
-      if (t + 1 < hi) issue(l, s.m1, s.n1, t + 2 >= hi);
-      multiply(acc, s.m0, s.n0);
-      if (t + 1 >= hi) break;
-      dma_wait();
-      __syncthreads();
-      if (t + 2 < hi) issue(l, s.m0, s.n0, t + 3 >= hi);
-      multiply(acc, s.m1, s.n1);
+    Frags f;
+    f.om = lane_offset<BM, MT>(this->wm * MI * 16);
+    f.on = lane_offset<BN, NT>(this->wn * NI * 16);
+    step<true>(acc, f, l, s.m0, s.n0, s.m1, s.n1, hi - lo);
+    int left = hi - lo - 1;
+    for (; left > 1; left -= 2) {
+      step<false>(acc, f, l, s.m1, s.n1, s.m0, s.n0, left);
+      step<false>(acc, f, l, s.m0, s.n0, s.m1, s.n1, left - 1);
     }
+    if (left > 0) step<false>(acc, f, l, s.m1, s.n1, s.m0, s.n0, 1);
+    multiply<3>(acc, f);
     __syncthreads();
   }
 };
@@ -268,6 +340,31 @@ struct SplitLoader {
   // base: the tile's first element at this step; rows past valid and k past left are zeros, and so are the k
   // whose `live` factor is 0 (turned only; live at this step).
   __device__ __forceinline__ void load(const float* base, int64_t ld, int valid, int left, const float* live) {
+    if (valid >= R && left >= 32) {  // uniform: a whole tile, without a test per value
+#pragma unroll
+      for (int t = 0; t < kTasks; ++t) {
+        const int r = row_of(t), k = 8 * chunk_of(t);
+        if constexpr (!TURNED) {
+          const float* p = base + r * ld + k;
+          __builtin_memcpy(&v[t][0], p, 16);
+          __builtin_memcpy(&v[t][4], p + 4, 16);
+        } else {
+          const float* p = base + k * ld + r;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[t][j] = p[j * ld];
+        }
+      }
+      if (TURNED && live) {  // uniform
+#pragma unroll
+        for (int t = 0; t < kTasks; ++t) {
+          float f[8];
+          __builtin_memcpy(f, live + 8 * chunk_of(t), 32);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[t][j] = f[j] != 0.f ? v[t][j] : 0.f;
+        }
+      }
+      return;
+    }
 #pragma unroll
     for (int t = 0; t < kTasks; ++t) {
       const int r = row_of(t), k = 8 * chunk_of(t);
@@ -387,6 +484,119 @@ struct SplitProduct : TileBase<BM_, BN_, WM_, WN_, 32> {
       multiply(acc, s.m, s.n);
       __syncthreads();
     }
+  }
+};
+
+// Small products: 32 x 32 tiles of operands that are k-contiguous, for few
+// tokens or few tiles, where what counts is the way of one load after another.
+// Four waves take every fourth 32 k each and load their fragments straight
+// from global memory, kAhead steps at a time (no LDS, no barrier); their sums
+// meet in LDS at the end, where each wave gets one 16 x 16 quarter.  fp32: the
+// part products of three magnitudes are summed apart.
+template <typename T>
+struct DirectProduct : TileBase<32, 32, 2, 2, 32> {
+  typedef TileBase<32, 32, 2, 2, 32> B;
+  static constexpr bool kSplit = sizeof(T) == 4;
+  static constexpr int kSums = kSplit ? 3 : 1;
+  static constexpr int kAhead = kSplit ? 2 : 4;
+  static constexpr int kBytesM = 4 * 4096, kBytesN = 16;
+
+  struct Lds {
+    char *m, *n;
+  };
+  struct Raw {
+    T v[8];
+  };
+
+  __device__ __forceinline__ DirectProduct(int m0, int n0, int M, int N) : B(m0, n0, M, N) {}
+
+  // Eight values at p; those past `left` (or of a row that does not exist) are zeros.
+  static __device__ __forceinline__ Raw fetch(const T* p, bool in, int left) {
+    Raw r;
+    if (in && left >= 8) {
+      __builtin_memcpy(r.v, p, sizeof(r.v));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) r.v[j] = in && j < left ? p[j] : (T)0.f;
+    }
+    return r;
+  }
+
+  __device__ __forceinline__ void run(f32x4 (&out)[1][1], const SegList& l, int, int, const Lds& s) {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    f32x4 acc[kSums][2][2];
+#pragma unroll
+    for (int a = 0; a < kSums; ++a)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[a][i >> 1][i & 1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int sg = 0; sg < l.n; ++sg) {
+      const Seg& q = l.s[sg];
+      const T *pm[2], *pn[2];
+      bool im[2], in[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        im[i] = 16 * i + c < this->mrows;
+        in[i] = 16 * i + c < this->nrows;
+        pm[i] = (const T*)q.m + (int64_t)(this->m0 + 16 * i + c) * q.ldm;
+        pn[i] = (const T*)q.n + (int64_t)(this->n0 + 16 * i + c) * q.ldn;
+      }
+      for (int k0 = 32 * this->wave; k0 < q.k; k0 += 128 * kAhead) {
+        Raw rm[kAhead][2], rn[kAhead][2];
+#pragma unroll
+        for (int t = 0; t < kAhead; ++t)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int k = k0 + 128 * t + 8 * g;
+            rm[t][i] = fetch(pm[i] + k, im[i], q.k - k);
+            rn[t][i] = fetch(pn[i] + k, in[i], q.k - k);
+          }
+#pragma unroll
+        for (int t = 0; t < kAhead; ++t) {
+          if constexpr (!kSplit) {
+            typename Elem<T>::frag fm[2], fn[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              __builtin_memcpy(&fm[i], rm[t][i].v, 16);
+              __builtin_memcpy(&fn[i], rn[t][i].v, 16);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              acc[0][i >> 1][i & 1] = Elem<T>::mma(acc[0][i >> 1][i & 1], fm[i >> 1], fn[i & 1]);
+          } else {
+            SplitFrag fm[2], fn[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              fm[i] = split8(rm[t][i].v);
+              fn[i] = split8(rn[t][i].v);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const SplitFrag &x = fm[i >> 1], &y = fn[i & 1];
+              f32x4 &lo = acc[2][i >> 1][i & 1], &mid = acc[1][i >> 1][i & 1], &hi = acc[0][i >> 1][i & 1];
+              lo = Elem<__bf16>::mma(lo, x.l, y.h);
+              lo = Elem<__bf16>::mma(lo, x.h, y.l);
+              lo = Elem<__bf16>::mma(lo, x.m, y.m);
+              mid = Elem<__bf16>::mma(mid, x.m, y.h);
+              mid = Elem<__bf16>::mma(mid, x.h, y.m);
+              hi = Elem<__bf16>::mma(hi, x.h, y.h);
+            }
+          }
+        }
+      }
+    }
+    // wave w keeps quarter (w % 2, w / 2): the four waves' sums of it, in wave order
+    f32x4* p = (f32x4*)s.m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f32x4 v = acc[0][i & 1][i >> 1];
+      if constexpr (kSplit) v += acc[1][i & 1][i >> 1] + acc[2][i & 1][i >> 1];
+      p[(i * 4 + this->wave) * 64 + lane] = v;
+    }
+    __syncthreads();
+    out[0][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) out[0][0] += p[(this->wave * 4 + w) * 64 + lane];
+    __syncthreads();
   }
 };
 

@@ -25,7 +25,10 @@
 // the largest |c|, so that rows which count alike are rounded like p - 1_t
 // itself (one c for all would round the targets' entries, near -c, all to the
 // same side).  fp16: the same with the largest entry at kF16Scale, since a
-// softmax over a large vocabulary is below fp16's smallest values.
+// softmax over a large vocabulary is below fp16's smallest values.  What the
+// rounding takes from a row's target, its largest entry as a rule, is kept in
+// fp32 and comes back, times the target's row of W (or B), where the sums over
+// the vocabulary are stored.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <string.h>
@@ -40,6 +43,10 @@ namespace {
 constexpr float kF16Scale = 16384.f;  // the largest stored magnitude: room below fp16's 65504 for rounding
 
 __host__ __device__ __forceinline__ int round8(int x) { return (x + 7) & ~7; }
+// Row stride of G and H of m columns: whole 128-byte lines, an odd number of
+// them.  With a power of two the 256 rows that a tile reads at once lie on a
+// few channels of the memory (8192 x 4096 x 32768 bf16 dX: 2281 us).
+__host__ __device__ __forceinline__ int piece_ld(int m) { return ((m + 63) / 64 | 1) * 64; }
 
 // ---------------------------------------------------------------------------
 // Row copies of 16-bit operands: padded to 8 columns (zeros), and zeros in the
@@ -74,25 +81,38 @@ __global__ __launch_bounds__(256) void k_copy_rows(CopyArgs a) {
 // ---------------------------------------------------------------------------
 // The products' tile shapes.  16-bit: 256 x 256 (eight waves of 128 x 64) and
 // 128 x 128 (four of 64 x 64); two accumulators: 256 x 128 (eight of 64 x 64)
-// and 128 x 128.  fp32: 128 x 128 (eight of 64 x 32), either way.
+// and 128 x 128.  fp32: 128 x 128 (eight of 64 x 32) and 64 x 128 (four of
+// 32 x 64).  Logits of few tokens or few tiles: 32 x 32 (DirectProduct).
 // ---------------------------------------------------------------------------
-template <typename T, bool MT, bool NT, bool DUAL, bool BIG>
+enum : int { kDirect = 0, kSmall = 1, kBig = 2 };
+
+template <typename T, bool MT, bool NT, bool DUAL, int SIZE>
 struct ProductOf {
-  static constexpr int BM = BIG ? 256 : 128, BN = BIG && !DUAL ? 256 : 128;
-  static constexpr int WM = DUAL && BIG ? 4 : 2, WN = DUAL && BIG ? 2 : BIG ? 4 : 2;
+  static constexpr bool big = SIZE == kBig;
+  static constexpr int BM = big ? 256 : 128, BN = big && !DUAL ? 256 : 128;
+  static constexpr int WM = DUAL && big ? 4 : 2, WN = DUAL && big ? 2 : big ? 4 : 2;
   typedef TileProduct<T, BM, BN, WM, WN, MT, NT> type;
 };
-template <bool MT, bool NT, bool DUAL, bool BIG>
-struct ProductOf<float, MT, NT, DUAL, BIG> {
-  typedef SplitProduct<128, 128, 2, 4, MT, NT> type;
+template <bool MT, bool NT, bool DUAL, int SIZE>
+struct ProductOf<float, MT, NT, DUAL, SIZE> {
+  static constexpr bool big = SIZE == kBig;
+  typedef SplitProduct<big ? 128 : 64, 128, 2, big ? 4 : 2, MT, NT> type;
+};
+template <typename T, bool DUAL>
+struct ProductOf<T, false, false, DUAL, kDirect> {
+  typedef DirectProduct<T> type;
+};
+template <bool DUAL>
+struct ProductOf<float, false, false, DUAL, kDirect> {
+  typedef DirectProduct<float> type;
 };
 
-template <typename T, bool BIG>
-constexpr int kThreadsOf = sizeof(T) == 4 || BIG ? 512 : 256;
+template <typename T, int SIZE>
+constexpr int kThreadsOf = SIZE == kBig ? 512 : 256;
 
 template <typename T, typename P>
 __device__ __forceinline__ typename P::Lds lds_of() {
-  if constexpr (sizeof(T) == 2) {
+  if constexpr (sizeof(T) == 2 && P::BM > 32) {
     __shared__ __attribute__((aligned(16))) char m0[P::kBytesM], m1[P::kBytesM], n0[P::kBytesN], n1[P::kBytesN];
     return {m0, m1, n0, n1};
   } else {
@@ -103,7 +123,7 @@ __device__ __forceinline__ typename P::Lds lds_of() {
 
 template <typename T, typename P>
 __device__ __forceinline__ P product_at(int m0, int n0, int M, int N, const float* live) {
-  if constexpr (sizeof(T) == 2) return P(m0, n0, M, N);
+  if constexpr (sizeof(T) == 2 || P::BM == 32) return P(m0, n0, M, N);
   else return P(m0, n0, M, N, live);
 }
 
@@ -122,27 +142,32 @@ struct ZArgs {
   float2* part;       // [parts][N]: (max, sum) | (sum p U, -)
   float* at_target;   // [N]: z or U at the target
   const float* h;     // [N]
+  const float* q;     // [N]: h - U at the target
   const float* colmul;  // [N]
-  void *g, *hh;       // G and H, [N][round8(M)], or null
+  float *rest_g, *rest_h;  // [N]: what rounding took from G and H at the target (16-bit)
+  void *g, *hh;       // G and H, [N][piece_ld(M)], or null
 };
 
-// A wave's tile to the rows of a [N][round8(M)] matrix.  val(i, j): the lane's
+// A wave's tile to the rows of a [N][piece_ld(M)] matrix.  val(i, j): the lane's
 // four values of acc[i][j], 0 past M.  16-bit: through the wave's own LDS, so
 // that global stores are whole 128-byte rows.
 template <typename P, typename T, typename F>
 __device__ __forceinline__ void store_tile(const P& tp, char* lds, void* out, int M, int N, F val) {
   constexpr int MI = P::MI, NI = P::NI;
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-  const int ld = round8(M);
+  const int ld = piece_ld(M);
   T* o = (T*)out;
-  if constexpr (sizeof(T) == 4) {
+  if constexpr (sizeof(T) == 4 || MI == 1) {
 #pragma unroll
     for (int j = 0; j < NI; ++j)
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
         const int n = tp.n_of(j), m = tp.m_of(i);
         const f32x4 v = val(i, j);
-        if (n < N && m < ld) *(f32x4*)(o + (int64_t)n * ld + m) = v;
+        if (n < N && m < ld) {
+          const T q[4] = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+          __builtin_memcpy(o + (int64_t)n * ld + m, q, sizeof(q));
+        }
       }
   } else {
     constexpr int RB = MI * 32, CH = RB / 16;  // row bytes, chunks
@@ -167,10 +192,10 @@ __device__ __forceinline__ void store_tile(const P& tp, char* lds, void* out, in
   }
 }
 
-template <typename T, int MODE, bool BIG>
-__global__ __launch_bounds__((kThreadsOf<T, BIG>)) void k_logits(ZArgs a) {
+template <typename T, int MODE, int SIZE>
+__global__ __launch_bounds__((kThreadsOf<T, SIZE>), 2) void k_logits(ZArgs a) {
   constexpr bool kDual = MODE >= kHSum;
-  typedef typename ProductOf<T, false, false, kDual, BIG>::type P;
+  typedef typename ProductOf<T, false, false, kDual, SIZE>::type P;
   constexpr int MI = P::MI, NI = P::NI;
   const typename P::Lds lds = lds_of<T, P>();
   int tm, tn;
@@ -212,7 +237,7 @@ __global__ __launch_bounds__((kThreadsOf<T, BIG>)) void k_logits(ZArgs a) {
     } else {
       const float mx = nin ? a.stat[n] : 0.f, inv = nin ? a.stat[a.N + n] : 0.f;
       const float cm = MODE != kHSum && nin ? a.colmul[n] : 0.f;
-      const float h = MODE == kHGrad && nin ? a.h[n] : 0.f;
+      const float h = MODE == kHGrad && nin ? a.h[n] : 0.f, q = MODE == kHGrad && nin ? a.q[n] : 0.f;
       float hs = 0.f;
 #pragma unroll
       for (int i = 0; i < MI; ++i)
@@ -226,8 +251,13 @@ __global__ __launch_bounds__((kThreadsOf<T, BIG>)) void k_logits(ZArgs a) {
             hs += in ? p * u[i][j][e] : 0.f;
             if (m == t) a.at_target[n] = u[i][j][e];
           } else {
-            if constexpr (MODE == kHGrad) u[i][j][e] = in ? cm * p * (u[i][j][e] - h) : 0.f;
+            // at the target from q: U there and h come from different sums, and p near 1 has their difference small
+            if constexpr (MODE == kHGrad) u[i][j][e] = in ? cm * p * (m == t ? -q : u[i][j][e] - h) : 0.f;
             z[i][j][e] = in ? cm * (m == t ? p - 1.f : p) : 0.f;
+            if (sizeof(T) == 2 && m == t) {
+              if (a.rest_g) a.rest_g[n] = z[i][j][e] - (float)(T)z[i][j][e];
+              if (MODE == kHGrad && a.rest_h) a.rest_h[n] = u[i][j][e] - (float)(T)u[i][j][e];
+            }
           }
         }
       if constexpr (MODE == kHSum) {
@@ -238,12 +268,34 @@ __global__ __launch_bounds__((kThreadsOf<T, BIG>)) void k_logits(ZArgs a) {
   }
   if constexpr (MODE == kGrad || MODE == kHGrad) {
     char* at;
-    if constexpr (sizeof(T) == 2) at = lds.m0;
+    if constexpr (sizeof(T) == 2 && SIZE != kDirect) at = lds.m0;
     else at = lds.m;
     if constexpr (kDual)
       if (a.hh) store_tile<P, T>(tp, at, a.hh, a.M, a.N, [&](int i, int j) { return u[i][j]; });
     if (a.g) store_tile<P, T>(tp, at, a.g, a.M, a.N, [&](int i, int j) { return z[i][j]; });
   }
+}
+
+// Rows of W and B at the targets, times what rounding took there.
+struct Rest {
+  const int64_t* target;
+  int V;
+  const void *w, *b;  // or null
+  int64_t ldw, ldb;
+  const float *rw, *rb;
+};
+
+template <typename T>
+__device__ __forceinline__ float rest_at(const Rest& a, int n, int m) {
+  float v = 0.f;
+  if constexpr (sizeof(T) == 2) {
+    const int64_t t = a.target ? a.target[n] : -1;
+    if (t >= 0 && t < a.V) {
+      if (a.w) v += a.rw[n] * (float)((const T*)a.w)[t * a.ldw + m];
+      if (a.b) v += a.rb[n] * (float)((const T*)a.b)[t * a.ldb + m];
+    }
+  }
+  return v;
 }
 
 // ---------------------------------------------------------------------------
@@ -262,11 +314,12 @@ struct OutArgs {
   const float* rows;  // [N] or null: rows that do not count (0) are 0
   const float* live;  // turned fp32 M operand: the k that do not count are left out
   const float* alpha;
+  Rest rest;
 };
 
-template <typename T, bool NT, bool BIG>
-__global__ __launch_bounds__((kThreadsOf<T, BIG>)) void k_product(OutArgs a) {
-  typedef typename ProductOf<T, true, NT, false, BIG>::type P;
+template <typename T, bool NT, int SIZE>
+__global__ __launch_bounds__((kThreadsOf<T, SIZE>)) void k_product(OutArgs a) {
+  typedef typename ProductOf<T, true, NT, false, SIZE>::type P;
   constexpr int MI = P::MI, NI = P::NI;
   const typename P::Lds lds = lds_of<T, P>();
   const int s = blockIdx.x / (a.tm * a.tn), id = blockIdx.x % (a.tm * a.tn);
@@ -300,6 +353,8 @@ __global__ __launch_bounds__((kThreadsOf<T, BIG>)) void k_product(OutArgs a) {
           for (int e = 0; e < cnt; ++e) o[e] = a.add ? o[e] + v[e] : v[e];
         }
       } else {
+        if constexpr (!NT)
+          for (int e = 0; e < cnt; ++e) v[e] += rest_at<T>(a.rest, n, m + e);
         v = dead ? f32x4{0.f, 0.f, 0.f, 0.f} : v * al;
         T* o = (T*)a.out + (int64_t)n * a.ld + m;
         float* o32 = a.out32 ? a.out32 + (int64_t)n * a.M + m : nullptr;
@@ -338,6 +393,7 @@ __global__ __launch_bounds__(256) void k_finish(OutArgs a) {
   }
   int n = (int)(i4 / a.M), m = (int)(i4 % a.M);
   if (cnt == 4 && m + 4 <= a.M) {
+    for (int e = 0; e < 4; ++e) v[e] += rest_at<T>(a.rest, n, m + e);
     v = a.rows && a.rows[n] == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : v * al;
     const T r[4] = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
     __builtin_memcpy((T*)a.out + n * a.ld + m, r, sizeof(r));
@@ -345,7 +401,7 @@ __global__ __launch_bounds__(256) void k_finish(OutArgs a) {
     return;
   }
   for (int e = 0; e < cnt; ++e) {
-    const float r = a.rows && a.rows[n] == 0.f ? 0.f : v[e] * al;
+    const float r = a.rows && a.rows[n] == 0.f ? 0.f : (v[e] + rest_at<T>(a.rest, n, m)) * al;
     ((T*)a.out)[n * a.ld + m] = (T)r;
     if (a.out32) a.out32[i4 + e] = r;
     if (++m == a.M) {
@@ -369,7 +425,7 @@ struct RowArgs {
   float* stat;  // [2N + 2]: max, 1/sum, 1/denominator, weight sum
   float* row;   // [N]: the rows' losses | the rows' shares of the upstream gradient's gradient
   float* out;   // reduced
-  float* h;
+  float *h, *q;
   float *coef, *live, *colmul, *alpha;
   const float *nx, *na, *nw, *nb;  // row norms of X, A, W, B (fp16 gg), or null
 };
@@ -409,18 +465,39 @@ __device__ __forceinline__ float2 join_parts(const float2* part, int parts, int 
   return s;
 }
 
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+  return v;
+}
+
+// The sums of the rows' losses and weights to the loss and its denominator.
+__device__ __forceinline__ void finish_loss(const RowArgs& a, float l, float w) {
+  if (threadIdx.x != 0) return;
+  const float inv = a.reduction == TTT_REDUCE_MEAN ? 1.f / fmaxf(w, 1.f) : 1.f;
+  a.stat[2 * a.N] = inv;
+  a.stat[2 * a.N + 1] = w;
+  if (a.reduction != TTT_REDUCE_NONE) a.out[0] = l * inv;
+}
+
 // The tiles' (max, sum) to the row's, and its loss: log(sum) - (z_t - max),
 // which keeps its digits where the target has nearly all of the probability.
 __global__ __launch_bounds__(1024) void k_join_loss(RowArgs a) {
   __shared__ float2 lds[16][64];
   const int n = blockIdx.x * 64 + (threadIdx.x & 63);
   const float2 s = join_parts<true>(a.part, a.parts, a.N, n, lds);
-  if (threadIdx.x >= 64 || n >= a.N) return;
-  a.stat[n] = s.x;
-  a.stat[a.N + n] = 1.f / s.y;
-  const float w = row_weight(a, n);
-  const float l = bad_target(a, n) ? __builtin_nanf("") : logf(s.y) - (a.at_target[n] - s.x);
-  a.row[n] = w == 0.f ? 0.f : w * l;
+  if (threadIdx.x >= 64) return;
+  float w = 0.f, wl = 0.f;
+  if (n < a.N) {
+    a.stat[n] = s.x;
+    a.stat[a.N + n] = 1.f / s.y;
+    w = row_weight(a, n);
+    const float l = bad_target(a, n) ? __builtin_nanf("") : logf(s.y) - (a.at_target[n] - s.x);
+    wl = w == 0.f ? 0.f : w * l;
+    a.row[n] = wl;
+  }
+  // up to 64 rows: the whole reduction is here
+  if (gridDim.x == 1) finish_loss(a, wave_sum(wl), wave_sum(w));
 }
 
 // h = sum p U, and the rows' shares of the upstream gradient's gradient.
@@ -430,6 +507,7 @@ __global__ __launch_bounds__(1024) void k_join_h(RowArgs a) {
   const float2 s = join_parts<false>(a.part, a.parts, a.N, n, lds);
   if (threadIdx.x >= 64 || n >= a.N) return;
   a.h[n] = s.x;
+  a.q[n] = s.x - a.at_target[n];
   if (a.row) {
     const float w = row_weight(a, n);
     a.row[n] = w == 0.f ? 0.f
@@ -482,12 +560,7 @@ __global__ __launch_bounds__(1024) void k_reduce_loss(RowArgs a) {
     }
   l = block_sum(l, lds);
   w = block_sum(w, lds);
-  if (threadIdx.x == 0) {
-    const float inv = a.reduction == TTT_REDUCE_MEAN ? 1.f / fmaxf(w, 1.f) : 1.f;
-    a.stat[2 * a.N] = inv;
-    a.stat[2 * a.N + 1] = w;
-    if (a.reduction != TTT_REDUCE_NONE) a.out[0] = l * inv;
-  }
+  finish_loss(a, l, w);
 }
 
 // The rows' coefficients c, which rows count, and the factors that G and H are stored with:
@@ -541,12 +614,6 @@ __global__ __launch_bounds__(1024) void k_sum(const float* x, int n, float* out)
   if (threadIdx.x == 0) *out = s;
 }
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
-  return v;
-}
-
 // norm[r] = |row r|, a wave a row.
 template <typename T>
 __global__ __launch_bounds__(256) void k_norms(const T* x, int64_t ld, int R, int C, float* norm) {
@@ -569,17 +636,19 @@ struct HArgs {
   int64_t ldx, ldw, lda, ldb;
   const float* dx32;  // [N][d]: the backward's dX (with a)
   const float* gb;    // [split][N][d]: G B (with b), over alpha
-  float* h;
+  const float* rest;  // [N]: what rounding took from G at the target, over alpha (16-bit)
+  float *h, *q;
 };
 
-// h_i = (A_i . dX_i + X_i . (G B)_i) / c_i + A_i . W_t + X_i . B_t: a wave a row.
+// q_i = (A_i . dX_i + X_i . (G B)_i) / c_i and h_i = q_i + A_i . W_t + X_i . B_t: a
+// wave a row.
 template <typename T>
 __global__ __launch_bounds__(256) void k_row_h(HArgs a) {
   const int n = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (n >= a.N) return;
   const float c = a.coef[n];
   if (!(c != 0.f) || c != c) {  // uniform: a row that does not count, or a target that does not exist
-    if (lane == 0) a.h[n] = 0.f;
+    if (lane == 0) a.h[n] = a.q[n] = 0.f;
     return;
   }
   const int64_t t = a.target[n], n64 = n;
@@ -595,13 +664,18 @@ __global__ __launch_bounds__(256) void k_row_h(HArgs a) {
       const float v = (float)((const T*)a.x)[n64 * a.ldx + i];
       float q = 0.f;
       for (int k = 0; k < a.split; ++k) q += a.gb[((int64_t)k * a.N + n64) * a.d + i];
+      const float bt = (float)((const T*)a.b)[t * a.ldb + i];
+      if (sizeof(T) == 2) q += a.rest[n] * bt;
       s += v * (q * al);
-      u += v * (float)((const T*)a.b)[t * a.ldb + i];
+      u += v * bt;
     }
   }
   s = wave_sum(s);
   u = wave_sum(u);
-  if (lane == 0) a.h[n] = s / c + u;
+  if (lane == 0) {
+    a.q[n] = s / c;
+    a.h[n] = s / c + u;
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -609,9 +683,9 @@ __global__ __launch_bounds__(256) void k_row_h(HArgs a) {
 // ---------------------------------------------------------------------------
 constexpr int64_t kPieceBytes = 512ll << 20;  // G (and H) of a piece
 constexpr int64_t kPackBytes = 256ll << 20;   // copied head rows of a forward piece
-constexpr int kMaxSplit = 16;
+constexpr int kMaxSplit = 64;
 constexpr int kMaxParts = 1024;    // rows of the tiles' partial results that are kept before they are merged
-constexpr int kStatsRows = 32768;  // vocabulary rows of a piece: at most kMaxParts / 2 such rows
+constexpr int kStatsRows = 32768;  // vocabulary rows of a piece at most
 
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -663,10 +737,28 @@ struct Carver {
   float* floats(int64_t n) { return (float*)take(n * 4); }
 };
 
-struct Spread {  // the tiles of a product and the workgroups of each
-  bool big;
-  int tm, tn, split, chunk;
+struct Spread {  // the tile shape of a product, and the workgroups of a tile
+  int size, split;
 };
+
+// A tile's rows along m, and tokens (or rows) along n.
+int tile_m(const Plan& k, int size) { return size == kDirect ? 32 : k.f32 ? (size == kBig ? 128 : 64) : size == kBig ? 256 : 128; }
+int tile_n(const Plan& k, int size, bool dual) { return size == kDirect ? 32 : !k.f32 && size == kBig && !dual ? 256 : 128; }
+
+// The tile shape of the logits: large where such tiles fill the card, direct
+// for a few tokens or few tiles.
+int logits_size(const Plan& k, bool dual, int M, int N) {
+  const auto tiles = [&](int size) { return cdiv(M, tile_m(k, size)) * cdiv(N, tile_n(k, size, dual)); };
+  if (N <= 32 || tiles(kSmall) < 96) return kDirect;
+  return tiles(kBig) >= (k.f32 ? 512 : 192) ? kBig : kSmall;
+}
+
+// Rows of parts that launch_logits writes for M vocabulary rows: one per wave
+// along them.
+int parts_of(const Plan& k, bool dual, int M, int N) {
+  const int size = logits_size(k, dual, M, N);
+  return (int)cdiv(M, tile_m(k, size)) * (dual && size == kBig && !k.f32 ? 4 : 2);
+}
 
 // The tile shape and split of a plain product of k in `segs` segments: the
 // least of (rounds of workgroups) x (steps of each) x (a step's time), plus the
@@ -675,21 +767,21 @@ struct Spread {  // the tiles of a product and the workgroups of each
 Spread spread_of(const Plan& p, int M, int N, int64_t k, bool keep) {
   const int step = p.f32 ? 32 : 64;
   const int steps = (int)cdiv(k, step);
-  Spread best{false, 0, 0, 0, 0};
+  Spread best{kSmall, 1};
   double least = 1e30;
-  for (int big = 0; big < (p.f32 ? 1 : 2); ++big) {
-    const int b = big ? 256 : 128, slots = big ? 256 : 512;
-    const double us = p.f32 ? 2.2 : big ? 1.8 : 1.4;
-    const int tm = (int)cdiv(M, b), tn = (int)cdiv(N, b);
-    for (int split = 1; split <= kMaxSplit; split += split < 4 ? 1 : 2) {
+  for (int size = kSmall; size <= kBig; ++size) {
+    const int slots = p.f32 ? (size == kBig ? 512 : 1024) : size == kBig ? 256 : 512;
+    const double us = p.f32 ? (size == kBig ? 3.2 : 3.4) : size == kBig ? 1.8 : 1.6;
+    const int64_t tiles = cdiv(M, tile_m(p, size)) * cdiv(N, tile_n(p, size, false));
+    for (int split = 1; split <= kMaxSplit; split += split < 4 ? 1 : split < 16 ? 2 : 8) {
       if (split > 1 && split * 4 > steps) break;
       const int chunk = (int)cdiv(steps, split);
-      const double rounds = (double)cdiv((int64_t)tm * tn * split, slots);
+      const double rounds = (double)cdiv(tiles * split, slots);
       double t = rounds * (chunk * us + 3);
       if (split > 1 || keep) t += 4 + 8.0 * split * M * N / 4e6;
       if (t < least) {
         least = t;
-        best = Spread{big != 0, tm, tn, (int)cdiv(steps, chunk), chunk};
+        best = Spread{size, (int)cdiv(steps, chunk)};
       }
     }
   }
@@ -706,7 +798,7 @@ struct Buffers {
   void *g, *hh;
   float *part_x, *part_w;  // fp32 parts of dx, dw
   float2* part;
-  float *at_target, *row, *h, *coef, *live, *colmul, *alpha, *nx, *na, *nw, *nb;
+  float *at_target, *row, *h, *q, *coef, *live, *colmul, *rest_g, *rest_h, *alpha, *nx, *na, *nw, *nb;
   int parts;
 };
 
@@ -715,8 +807,11 @@ Buffers layout(const Plan& k, Carver* c) {
   Buffers b;
   memset(&b, 0, sizeof(b));
   const bool fwd = k.entry == TTT_LCE_FWD, gg = k.entry == TTT_LCE_GG;
-  const int64_t each = cdiv(k.vc, 128) * 4;
-  if (fwd || gg) b.parts = (int)(each * k.pieces < each + kMaxParts ? each * k.pieces : each + kMaxParts);
+  if (fwd || gg) {
+    const int whole = parts_of(k, gg, k.vc, k.N), last = parts_of(k, gg, k.V - (k.pieces - 1) * k.vc, k.N);
+    const int64_t all = (int64_t)whole * (k.pieces - 1) + last;
+    b.parts = all <= kMaxParts ? (int)all : kMaxParts + (whole > last ? whole : last);
+  }
   if (b.parts) b.part = (float2*)c->take((int64_t)b.parts * k.N * 8);
   b.at_target = c->floats(k.N);
   b.row = c->floats(k.N);
@@ -731,11 +826,14 @@ Buffers layout(const Plan& k, Carver* c) {
   }
   if (fwd) return b;
   b.h = c->floats(k.N);
+  b.q = c->floats(k.N);
+  b.rest_g = c->floats(k.N);
+  b.rest_h = c->floats(k.N);
   b.coef = c->floats(k.N);
   b.live = c->floats(k.N);
   b.colmul = c->floats(k.N);
   b.alpha = c->floats(1);
-  const int64_t gb = (int64_t)k.es * k.N * round8(k.vc);
+  const int64_t gb = (int64_t)k.es * k.N * piece_ld(k.vc);
   b.g = c->take(gb);
   if (gg) {
     b.hh = c->take(gb);
@@ -781,34 +879,23 @@ void launch_copy(const void* src, int64_t ld, int R, int C, void* dst, const flo
   k_copy_rows<<<(unsigned)(n < 8192 ? n : 8192), 256, 0, st>>>(a);
 }
 
-// Tiles of 256 where there are enough of them to fill the card.
-bool big_logits(const Plan& k, bool dual, int M, int N) {
-  return !k.f32 && cdiv(M, 256) * cdiv(N, dual ? 128 : 256) >= 192;
-}
-
-// Rows of parts that launch_logits writes for M vocabulary rows: one per wave
-// along them.
-int parts_of(const Plan& k, bool dual, int M, int N) {
-  const bool big = big_logits(k, dual, M, N);
-  return (int)cdiv(M, big ? 256 : 128) * (big && dual ? 4 : 2);
-}
-
 template <int MODE>
 void launch_logits(const Plan& k, ZArgs a, hipStream_t st) {
   constexpr bool dual = MODE >= kHSum;
-  const bool big = big_logits(k, dual, a.M, a.N);
-  a.tm = (int)cdiv(a.M, big ? 256 : 128);
-  a.tn = (int)cdiv(a.N, big && !dual ? 256 : 128);
+  const int size = logits_size(k, dual, a.M, a.N);
+  a.tm = (int)cdiv(a.M, tile_m(k, size));
+  a.tn = (int)cdiv(a.N, tile_n(k, size, dual));
   const unsigned grid = (unsigned)(a.tm * a.tn);
-  if (k.dtype == TTT_F32) {
-    k_logits<float, MODE, false><<<grid, 512, 0, st>>>(a);
-  } else if (k.dtype == TTT_BF16) {
-    if (big) k_logits<__bf16, MODE, true><<<grid, 512, 0, st>>>(a);
-    else k_logits<__bf16, MODE, false><<<grid, 256, 0, st>>>(a);
-  } else {
-    if (big) k_logits<_Float16, MODE, true><<<grid, 512, 0, st>>>(a);
-    else k_logits<_Float16, MODE, false><<<grid, 256, 0, st>>>(a);
-  }
+#define LOGITS(T)                                                                     \
+  do {                                                                                \
+    if (size == kBig) k_logits<T, MODE, kBig><<<grid, 512, 0, st>>>(a);               \
+    else if (size == kSmall) k_logits<T, MODE, kSmall><<<grid, 256, 0, st>>>(a);      \
+    else k_logits<T, MODE, kDirect><<<grid, 256, 0, st>>>(a);                         \
+  } while (0)
+  if (k.dtype == TTT_F32) LOGITS(float);
+  else if (k.dtype == TTT_BF16) LOGITS(__bf16);
+  else LOGITS(_Float16);
+#undef LOGITS
 }
 
 // Makes room in part for the rows of a piece of m vocabulary rows.
@@ -820,15 +907,15 @@ void make_room(const Plan& k, const Buffers& b, int m, int* parts, hipStream_t s
 }
 
 template <typename T>
-void launch_product_of(const OutArgs& a, bool nt, bool big, bool fin, hipStream_t st) {
+void launch_product_of(const OutArgs& a, bool nt, int size, bool fin, hipStream_t st) {
   const unsigned grid = (unsigned)(a.tm * a.tn * a.split);
-  const unsigned threads = sizeof(T) == 4 || big ? 512 : 256;
-  if constexpr (sizeof(T) == 2) {
-    if (big && nt) k_product<T, true, true><<<grid, threads, 0, st>>>(a);
-    else if (big) k_product<T, false, true><<<grid, threads, 0, st>>>(a);
+  if (size == kBig) {
+    if (nt) k_product<T, true, kBig><<<grid, 512, 0, st>>>(a);
+    else k_product<T, false, kBig><<<grid, 512, 0, st>>>(a);
+  } else {
+    if (nt) k_product<T, true, kSmall><<<grid, 256, 0, st>>>(a);
+    else k_product<T, false, kSmall><<<grid, 256, 0, st>>>(a);
   }
-  if (!big && nt) k_product<T, true, false><<<grid, threads, 0, st>>>(a);
-  else if (!big) k_product<T, false, false><<<grid, threads, 0, st>>>(a);
   if (fin) k_finish<T><<<(unsigned)cdiv((int64_t)a.N * a.M, 1024), 256, 0, st>>>(a);
 }
 
@@ -840,15 +927,15 @@ void launch_product(const Plan& k, OutArgs a, bool nt, float* part, bool keep, c
                     hipStream_t st) {
   int steps = 0;
   for (int i = 0; i < a.l.n; ++i) steps += (int)cdiv(a.l.s[i].k, k.f32 ? 32 : 64);
-  a.tm = (int)cdiv(a.M, s.big ? 256 : 128);
-  a.tn = (int)cdiv(a.N, s.big ? 256 : 128);
+  a.tm = (int)cdiv(a.M, tile_m(k, s.size));
+  a.tn = (int)cdiv(a.N, tile_n(k, s.size, false));
   a.split = s.split;
   a.chunk = (int)cdiv(steps, s.split);
   a.part = keep || s.split > 1 ? part : nullptr;
   const bool fin = a.part && last;
-  if (k.dtype == TTT_F32) launch_product_of<float>(a, nt, false, fin, st);
-  else if (k.dtype == TTT_BF16) launch_product_of<__bf16>(a, nt, s.big, fin, st);
-  else launch_product_of<_Float16>(a, nt, s.big, fin, st);
+  if (k.dtype == TTT_F32) launch_product_of<float>(a, nt, s.size, fin, st);
+  else if (k.dtype == TTT_BF16) launch_product_of<__bf16>(a, nt, s.size, fin, st);
+  else launch_product_of<_Float16>(a, nt, s.size, fin, st);
 }
 
 int check(const ttt_lce_problem* p) {
@@ -921,6 +1008,7 @@ RowArgs row_args(const ttt_lce_problem* p, const Plan& k, const Buffers& b, cons
   r.part = b.part;
   r.at_target = b.at_target;
   r.h = b.h;
+  r.q = b.q;
   r.coef = b.coef;
   r.live = b.live;
   r.colmul = b.colmul;
@@ -964,14 +1052,18 @@ struct Call {
     a.target = target;
     a.stat = stat;
     a.h = b.h;
+    a.q = b.q;
     a.colmul = b.colmul;
+    a.rest_g = b.rest_g;
+    a.rest_h = b.rest_h;
     return a;
   }
   // Operands that are G or H of a piece of m rows
-  Operand piece(const void* g, int m) const { return {g, round8(m)}; }
+  Operand piece(const void* g, int m) const { return {g, piece_ld(m)}; }
 
   // out [N, d] (+)= the list's product over the piece
-  void over_vocab(const SegList& l, const ttt_rows* out, float* out32, bool add, bool keep, bool last) const {
+  void over_vocab(const SegList& l, const ttt_rows* out, float* out32, bool add, bool keep, bool last,
+                  const Rest& rest) const {
     OutArgs o;
     memset(&o, 0, sizeof(o));
     o.l = l;
@@ -983,6 +1075,7 @@ struct Call {
     }
     o.out32 = out32;
     o.rows = b.live;
+    o.rest = rest;
     o.alpha = b.alpha;
     o.add = add;
     launch_product(k, o, false, b.part_x, keep, spread_x(k, l.n, keep), last, st);
@@ -1051,7 +1144,7 @@ int ttt_lce_fwd(const ttt_lce_problem* p, const ttt_rows* x, const ttt_rows* w, 
   r.row = p->reduction == TTT_REDUCE_NONE ? loss : b.row;
   r.out = loss;
   k_join_loss<<<(unsigned)cdiv(k.N, 64), 1024, 0, st>>>(r);
-  k_reduce_loss<<<1, 1024, 0, st>>>(r);
+  if (k.N > 64) k_reduce_loss<<<1, 1024, 0, st>>>(r);
   return finish("ttt_lce_fwd");
 }
 
@@ -1085,7 +1178,8 @@ int ttt_lce_bwd(const ttt_lce_problem* p, const ttt_rows* x, const ttt_rows* w, 
     if (want_x) {
       SegList l{};
       add_product(&l, wo, go, m);
-      call.over_vocab(l, dx, dx32, v0 > 0, k.pieces > 1, v0 + m >= k.V);
+      call.over_vocab(l, dx, dx32, v0 > 0, k.pieces > 1, v0 + m >= k.V,
+                      Rest{target, k.V, w->data, nullptr, w->stride, 0, b.rest_g, nullptr});
     }
     if (want_w) {
       SegList l{};
@@ -1178,11 +1272,12 @@ int ttt_lce_gg(const ttt_lce_problem* p, const ttt_rows* x, const ttt_rows* w, c
         launch_logits<kGrad>(k, a, st);
         SegList l{};
         add_product(&l, rows_of(k, cb, v0, m, b.br, true, st), call.piece(b.g, m), m);
-        call.over_vocab(l, nullptr, nullptr, v0 > 0, true, false);
+        call.over_vocab(l, nullptr, nullptr, v0 > 0, true, false, Rest{});
       }
       walked = true;
       h.gb = b.part_x;
       h.split = spread_x(k, 1, true).split;
+      h.rest = b.rest_g;
       h.b = cb->data;
       h.ldb = cb->stride;
     }
@@ -1202,6 +1297,7 @@ int ttt_lce_gg(const ttt_lce_problem* p, const ttt_rows* x, const ttt_rows* w, c
     h.w = w->data;
     h.ldw = w->stride;
     h.h = b.h;
+    h.q = b.q;
     const unsigned grid = (unsigned)cdiv(k.N, 4);
     if (k.dtype == TTT_F32) k_row_h<float><<<grid, 256, 0, st>>>(h);
     else if (k.dtype == TTT_BF16) k_row_h<__bf16><<<grid, 256, 0, st>>>(h);
@@ -1222,7 +1318,9 @@ int ttt_lce_gg(const ttt_lce_problem* p, const ttt_rows* x, const ttt_rows* w, c
       SegList l{};
       add_product(&l, rows_of(k, w, v0, m, b.wr, false, st), ho, m);
       if (has_b && sums) add_product(&l, rows_of(k, cb, v0, m, b.br, false, st), go, m);
-      call.over_vocab(l, gx, nullptr, v0 > 0 || kept, k.pieces > 1 || kept, v0 + m >= k.V);
+      call.over_vocab(l, gx, nullptr, v0 > 0 || kept, k.pieces > 1 || kept, v0 + m >= k.V,
+                      Rest{target, k.V, w->data, has_b ? cb->data : nullptr, w->stride, has_b ? cb->stride : 0,
+                           b.rest_h, b.rest_g});
     }
     if (want_w) {
       SegList l{};
