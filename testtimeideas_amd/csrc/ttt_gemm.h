@@ -23,9 +23,10 @@
 // SplitProduct (fp32): a value is the sum of three bf16 parts, exactly
 // (split_pair), and a product the sum of the six part products above 2^-22 of
 // it, smallest first, in fp32: six times the matrix work of bf16, where the
-// fp32 instruction takes sixteen.  A step is 32 k: values go to registers one
-// step ahead, are split once and stored as three tiles of parts; either order
-// of an operand ends up the same there.
+// fp32 instruction takes sixteen.  A step is 32 k: values go to registers two
+// steps ahead, are split once, among the products of the step before theirs,
+// and stored as three tiles of parts; either order of an operand ends up the
+// same there.
 #pragma once
 
 #include "ttt_common.h"
@@ -326,6 +327,7 @@ struct SplitLoader {
   static_assert(!TURNED || kTasks % 2 == 0 || kTasks == 1, "tile shape");
   static constexpr int kPlane = R * 64;  // bytes of a part's tile
   float v[kTasks][8];
+  float f[kTasks][8];  // LIVE: the k's factors
 
   // Row and chunk of a task.  plain: four lanes share a row's 128 bytes;
   // turned: neighbouring lanes have neighbouring rows.
@@ -337,40 +339,16 @@ struct SplitLoader {
     const int i = (int)threadIdx.x + t * THREADS;
     return TURNED ? i / R : i & 3;
   }
-  // base: the tile's first element at this step; rows past valid and k past left are zeros, and so are the k
-  // whose `live` factor is 0 (turned only; live at this step).
+  // base: the tile's first element at this step; rows past valid and k past left are zeros, and so, with LIVE,
+  // are the k whose `live` factor is 0 (live at this step).  WHOLE: nothing is past anything.
+  template <bool WHOLE, bool LIVE>
   __device__ __forceinline__ void load(const float* base, int64_t ld, int valid, int left, const float* live) {
-    if (valid >= R && left >= 32) {  // uniform: a whole tile, without a test per value
-#pragma unroll
-      for (int t = 0; t < kTasks; ++t) {
-        const int r = row_of(t), k = 8 * chunk_of(t);
-        if constexpr (!TURNED) {
-          const float* p = base + r * ld + k;
-          __builtin_memcpy(&v[t][0], p, 16);
-          __builtin_memcpy(&v[t][4], p + 4, 16);
-        } else {
-          const float* p = base + k * ld + r;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[t][j] = p[j * ld];
-        }
-      }
-      if (TURNED && live) {  // uniform
-#pragma unroll
-        for (int t = 0; t < kTasks; ++t) {
-          float f[8];
-          __builtin_memcpy(f, live + 8 * chunk_of(t), 32);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[t][j] = f[j] != 0.f ? v[t][j] : 0.f;
-        }
-      }
-      return;
-    }
 #pragma unroll
     for (int t = 0; t < kTasks; ++t) {
       const int r = row_of(t), k = 8 * chunk_of(t);
       if constexpr (!TURNED) {
         const float* p = base + r * ld + k;
-        if (r < valid && k + 8 <= left) {
+        if (WHOLE || (r < valid && k + 8 <= left)) {
           __builtin_memcpy(&v[t][0], p, 16);
           __builtin_memcpy(&v[t][4], p + 4, 16);
         } else {
@@ -380,11 +358,14 @@ struct SplitLoader {
       } else {
         const float* p = base + k * ld + r;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          v[t][j] = r < valid && k + j < left && (!live || live[k + j] != 0.f) ? p[j * ld] : 0.f;
+        for (int j = 0; j < 8; ++j) {
+          v[t][j] = WHOLE || (r < valid && k + j < left) ? p[j * ld] : 0.f;
+          if constexpr (LIVE) f[t][j] = WHOLE || k + j < left ? live[k + j] : 0.f;
+        }
       }
     }
   }
+  template <bool LIVE>
   __device__ __forceinline__ void store(char* lds) const {
 #pragma unroll
     for (int t = 0; t < kTasks; ++t) {
@@ -393,7 +374,12 @@ struct SplitLoader {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         uint32_t a, b, c;
-        split_pair(v[t][2 * j], v[t][2 * j + 1], a, b, c);
+        float x = v[t][2 * j], y = v[t][2 * j + 1];
+        if constexpr (LIVE) {
+          x = f[t][2 * j] != 0.f ? x : 0.f;
+          y = f[t][2 * j + 1] != 0.f ? y : 0.f;
+        }
+        split_pair(x, y, a, b, c);
         h[j] = a;
         m[j] = b;
         l[j] = c;
@@ -418,30 +404,55 @@ struct SplitProduct : TileBase<BM_, BN_, WM_, WN_, 32> {
   static constexpr int kBytesM = BM * 64 * 3, kBytesN = BN * 64 * 3;
 
   struct Lds {
-    char *m, *n;
+    char *m0, *m1, *n0, *n1;
+  };
+  struct Regs {  // a step's values
+    SplitLoader<BM, kThreads_, MT> m;
+    SplitLoader<BN, kThreads_, NT> n;
   };
 
-  SplitLoader<BM, kThreads_, MT> lm;
-  SplitLoader<BN, kThreads_, NT> ln;
   const float* live;  // factors of the k of a turned M operand, or null
 
   __device__ __forceinline__ SplitProduct(int m0, int n0, int M, int N, const float* live_)
       : B(m0, n0, M, N), live(live_) {}
 
-  // Load the current step's values and move to the next.
-  __device__ __forceinline__ void load(const SegList& l) {
+  // Both operands turned is a sum over the rows of X (or A): those that do not
+  // count are left out.
+  static constexpr bool kLive = MT && NT;
+
+  const float *bm, *bn;  // the tile's first elements at this step
+  int64_t ldm, ldn, incm, incn;
+  int kseg;
+
+  __device__ __forceinline__ void enter(const SegList& l) {
     const Seg& s = l.s[this->seg];
     const int64_t k0 = this->k0;
-    const int left = s.k - this->k0;
-    lm.load((const float*)s.m + (MT ? k0 * s.ldm + this->m0 : this->m0 * s.ldm + k0), s.ldm, this->mrows, left,
-            MT && live ? live + k0 : nullptr);
-    ln.load((const float*)s.n + (NT ? k0 * s.ldn + this->n0 : this->n0 * s.ldn + k0), s.ldn, this->nrows, left,
-            nullptr);
+    kseg = s.k;
+    ldm = s.ldm;
+    ldn = s.ldn;
+    incm = MT ? 32 * ldm : 32;
+    incn = NT ? 32 * ldn : 32;
+    bm = (const float*)s.m + (MT ? k0 * ldm + this->m0 : this->m0 * ldm + k0);
+    bn = (const float*)s.n + (NT ? k0 * ldn + this->n0 : this->n0 * ldn + k0);
+  }
+  // Load the current step's values and move to the next.
+  template <bool WHOLE>
+  __device__ __forceinline__ void load(const SegList& l, Regs& r) {
+    const int left = kseg - this->k0;
+    r.m.template load<WHOLE, kLive>(bm, ldm, this->mrows, left, kLive ? live + this->k0 : nullptr);
+    r.n.template load<WHOLE, false>(bn, ldn, this->nrows, left, nullptr);
     this->k0 += 32;
+    bm += incm;
+    bn += incn;
     if (left <= 32 && this->seg + 1 < l.n) {
       ++this->seg;
       this->k0 = 0;
+      enter(l);
     }
+  }
+  static __device__ __forceinline__ void store(const Regs& r, char* om, char* on) {
+    r.m.template store<kLive>(om);
+    r.n.template store<false>(on);
   }
 
   __device__ __forceinline__ void multiply(f32x4 (&acc)[MI][NI], const char* sm, const char* sn) const {
@@ -457,13 +468,21 @@ struct SplitProduct : TileBase<BM_, BN_, WM_, WN_, 32> {
 #pragma unroll
         for (int j = 0; j < NI; ++j) acc[i][j] = Elem<__bf16>::mma(acc[i][j], fm[a][i], fn[b][j]);
     };
+    // the reads in the order of their products
+    const auto read_m = [&](int a) {
 #pragma unroll
-    for (int a = 2; a >= 0; --a) {
+      for (int i = 0; i < MI; ++i) fm[a][i] = *(const bf16x8*)(pm + a * (BM * 64) + i * 1024);
+    };
+    const auto read_n = [&](int a) {
 #pragma unroll
-      for (int i = 0; i < MI; ++i) fm[a][i] = *(const bf16x8*)(pm + a * lm.kPlane + i * 1024);
-#pragma unroll
-      for (int j = 0; j < NI; ++j) fn[a][j] = *(const bf16x8*)(pn + a * ln.kPlane + j * 1024);
-    }
+      for (int j = 0; j < NI; ++j) fn[a][j] = *(const bf16x8*)(pn + a * (BN * 64) + j * 1024);
+    };
+    read_m(2);
+    read_n(0);
+    read_m(0);
+    read_n(2);
+    read_m(1);
+    read_n(1);
     part(2, 0);
     part(0, 2);
     part(1, 1);
@@ -472,18 +491,64 @@ struct SplitProduct : TileBase<BM_, BN_, WM_, WN_, 32> {
     part(0, 0);
   }
 
+  // The products of the step in (sm, sn), while the values of the next, in r
+  // (MORE > 0), are split and stored to (om, on) and those of the one after
+  // (MORE > 1) are on their way to q.
+  template <bool WHOLE, int MORE>
+  __device__ __forceinline__ void step(f32x4 (&acc)[MI][NI], const SegList& l, const char* sm, const char* sn,
+                                       char* om, char* on, const Regs& r, Regs& q) {
+    if constexpr (MORE > 1) {
+      load<WHOLE>(l, q);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    multiply(acc, sm, sn);
+    if constexpr (MORE > 0) {
+      store(r, om, on);
+      // all reads, some of the split's operations while the first arrive, then a few behind every product
+      __builtin_amdgcn_sched_group_barrier(0x100, 3 * (MI + NI), 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 16, 0);
+#pragma unroll
+      for (int i = 0; i < 6 * MI * NI; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+      }
+    }
+    __syncthreads();
+  }
+
+  // WHOLE: without a test, the number of loads on their way is known where the
+  // values of the step before are waited for, and only those are.
+  template <bool WHOLE>
+  __device__ __forceinline__ void walk(f32x4 (&acc)[MI][NI], const SegList& l, int steps, const Lds& s) {
+    Regs a, b;
+    load<WHOLE>(l, a);
+    store(a, s.m0, s.n0);
+    if (steps > 1) load<WHOLE>(l, b);
+    __syncthreads();
+    for (; steps > 3; steps -= 2) {
+      step<WHOLE, 2>(acc, l, s.m0, s.n0, s.m1, s.n1, b, a);
+      step<WHOLE, 2>(acc, l, s.m1, s.n1, s.m0, s.n0, a, b);
+    }
+    if (steps == 3) {
+      step<WHOLE, 2>(acc, l, s.m0, s.n0, s.m1, s.n1, b, a);
+      step<WHOLE, 1>(acc, l, s.m1, s.n1, s.m0, s.n0, a, b);
+      step<WHOLE, 0>(acc, l, s.m0, s.n0, s.m1, s.n1, a, b);
+    } else if (steps == 2) {
+      step<WHOLE, 1>(acc, l, s.m0, s.n0, s.m1, s.n1, b, a);
+      step<WHOLE, 0>(acc, l, s.m1, s.n1, s.m0, s.n0, a, b);
+    } else {
+      step<WHOLE, 0>(acc, l, s.m0, s.n0, s.m1, s.n1, a, b);
+    }
+  }
+
   __device__ __forceinline__ void run(f32x4 (&acc)[MI][NI], const SegList& l, int lo, int hi, const Lds& s) {
     if (lo >= hi) return;  // uniform
     this->seek(l, lo);
-    load(l);
-    for (int t = lo; t < hi; ++t) {
-      lm.store(s.m);
-      ln.store(s.n);
-      __syncthreads();
-      if (t + 1 < hi) load(l);
-      multiply(acc, s.m, s.n);
-      __syncthreads();
-    }
+    enter(l);
+    bool whole = this->mrows >= BM && this->nrows >= BN;
+    for (int i = 0; i < l.n; ++i) whole = whole && l.s[i].k % 32 == 0;
+    if (whole) walk<true>(acc, l, hi - lo, s);
+    else walk<false>(acc, l, hi - lo, s);
   }
 };
 

@@ -112,7 +112,7 @@ constexpr int kThreadsOf = SIZE == kBig ? 512 : 256;
 
 template <typename T, typename P>
 __device__ __forceinline__ typename P::Lds lds_of() {
-  if constexpr (sizeof(T) == 2 && P::BM > 32) {
+  if constexpr (P::BM > 32) {
     __shared__ __attribute__((aligned(16))) char m0[P::kBytesM], m1[P::kBytesM], n0[P::kBytesN], n1[P::kBytesN];
     return {m0, m1, n0, n1};
   } else {
@@ -268,7 +268,7 @@ __global__ __launch_bounds__((kThreadsOf<T, SIZE>), 2) void k_logits(ZArgs a) {
   }
   if constexpr (MODE == kGrad || MODE == kHGrad) {
     char* at;
-    if constexpr (sizeof(T) == 2 && SIZE != kDirect) at = lds.m0;
+    if constexpr (SIZE != kDirect) at = lds.m0;
     else at = lds.m;
     if constexpr (kDual)
       if (a.hh) store_tile<P, T>(tp, at, a.hh, a.M, a.N, [&](int i, int j) { return u[i][j]; });
@@ -318,7 +318,7 @@ struct OutArgs {
 };
 
 template <typename T, bool NT, int SIZE>
-__global__ __launch_bounds__((kThreadsOf<T, SIZE>)) void k_product(OutArgs a) {
+__global__ __launch_bounds__((kThreadsOf<T, SIZE>), 2) void k_product(OutArgs a) {
   typedef typename ProductOf<T, true, NT, false, SIZE>::type P;
   constexpr int MI = P::MI, NI = P::NI;
   const typename P::Lds lds = lds_of<T, P>();

@@ -14,6 +14,7 @@
 #include <string.h>
 
 #include "../../include/ttt_ops.h"
+#include "ttt_common.h"
 #include "ttt_ops.h"
 
 namespace ttt {
@@ -34,26 +35,31 @@ struct NormArgs {
 template <typename T>
 constexpr int kVec = 16 / (int)sizeof(T);
 
-// Eight (four) consecutive values at p as fp32; the loads are 16 bytes wide
-// whatever p's alignment is (global memory takes any).  Values past D read 0.
+// A chunk as it was loaded: eight 16-bit or four fp32 values.  The loads are 16
+// bytes wide whatever the address is (global memory takes any); values past D
+// read as 0.
 template <typename T>
-__device__ __forceinline__ void load_chunk(const T* row, int col, int D, float* v) {
+struct Raw {
+  T v[kVec<T>];
+};
+
+template <typename T, bool WHOLE>
+__device__ __forceinline__ Raw<T> load_raw(const T* row, int col, int D) {
   constexpr int V = kVec<T>;
-  T r[V];
-  if (col + V <= D) {
-    __builtin_memcpy(r, row + col, 16);
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = (float)r[j];
+  Raw<T> r;
+  if (WHOLE ? col < D : col + V <= D) {
+    __builtin_memcpy(r.v, row + col, 16);
   } else {
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = col + j < D ? (float)row[col + j] : 0.f;
+    for (int j = 0; j < V; ++j) r.v[j] = !WHOLE && col + j < D ? row[col + j] : (T)0.f;
   }
+  return r;
 }
 
-template <typename T>
+template <typename T, bool WHOLE>
 __device__ __forceinline__ void store_chunk(T* row, int col, int D, const float* v) {
   constexpr int V = kVec<T>;
-  if (col + V <= D) {
+  if (WHOLE ? col < D : col + V <= D) {
     T r[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) r[j] = (T)v[j];
@@ -61,12 +67,12 @@ __device__ __forceinline__ void store_chunk(T* row, int col, int D, const float*
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j)
-      if (col + j < D) row[col + j] = (T)v[j];
+      if (!WHOLE && col + j < D) row[col + j] = (T)v[j];
   }
 }
 
-// V parameters at column col: of type T, or fp32 (f32); `none` where p is null.
-template <typename T>
+// A chunk's parameters at column col: of type T, or fp32 (f32); `none` where p is null.
+template <typename T, bool WHOLE>
 __device__ __forceinline__ void load_param(const void* p, int f32, int col, int D, float none, float* v) {
   constexpr int V = kVec<T>;
   if (!p) {
@@ -77,26 +83,37 @@ __device__ __forceinline__ void load_param(const void* p, int f32, int col, int 
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] = col + j < D ? q[col + j] : 0.f;
   } else {
-    load_chunk<T>((const T*)p, col, D, v);
+    const Raw<T> r = load_raw<T, WHOLE>((const T*)p, col, D);
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = (float)r.v[j];
   }
 }
 
-__device__ __forceinline__ float lane_swap_sum(float x, int mask) {
-  return x + __shfl_xor(x, mask);
+// Sum over a wave, to every lane: lane swaps within 16 lanes (DPP: pairs,
+// halves of four, mirrored halves and rows), then across (group_sum).
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float x) {
+  return x + __uint_as_float(__builtin_amdgcn_mov_dpp((int)__float_as_uint(x), CTRL, 0xF, 0xF, true));
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  x = dpp_add<0xB1>(x);   // quad_perm 1,0,3,2
+  x = dpp_add<0x4E>(x);   // quad_perm 2,3,0,1
+  x = dpp_add<0x141>(x);  // row_half_mirror
+  x = dpp_add<0x140>(x);  // row_mirror
+  return group_sum(x);
 }
 
 // Sums of NS values over the threads of a row (TPR = 64: a wave; more: the
-// workgroup, through LDS), to every thread.
+// workgroup, through LDS, `turn` picking one of two places so that one barrier
+// does), to every thread.
 template <int TPR, int NS>
-__device__ __forceinline__ void row_sums(float* s, float* lds) {
+__device__ __forceinline__ void row_sums(float* s, float* lds, int turn) {
 #pragma unroll
-  for (int k = 0; k < NS; ++k)
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) s[k] = lane_swap_sum(s[k], m);
+  for (int k = 0; k < NS; ++k) s[k] = wave_sum(s[k]);
   if constexpr (TPR > 64) {
     constexpr int W = TPR / 64;
     const int w = threadIdx.x >> 6;
-    __syncthreads();  // the sums of the call before have been read
+    lds += turn * (NS * W);
     if ((threadIdx.x & 63) == 0)
 #pragma unroll
       for (int k = 0; k < NS; ++k) lds[k * W + w] = s[k];
@@ -111,63 +128,90 @@ __device__ __forceinline__ void row_sums(float* s, float* lds) {
   }
 }
 
-// Thread's chunk `ch` of a row: columns of chunk-major order, so a wave's
+// Thread's chunk `ch` of a row: columns in chunk-major order, so a wave's
 // loads of one chunk are contiguous.
 template <typename T, int TPR>
 __device__ __forceinline__ int chunk_col(int ch) {
   return (ch * TPR + (int)(threadIdx.x % TPR)) * kVec<T>;
 }
 
-template <typename T, int TPR, int NCH, int THREADS>
+// The chunks of a row of x; rows past the last are not read.
+template <typename T, int TPR, int NCH, bool WHOLE>
+__device__ __forceinline__ void load_row(const void* x, int64_t ld, int64_t row, const NormArgs& a, Raw<T>* r) {
+  if (row < a.N) {
+#pragma unroll
+    for (int ch = 0; ch < NCH; ++ch) r[ch] = load_raw<T, WHOLE>((const T*)x + row * ld, chunk_col<T, TPR>(ch), a.D);
+  }
+}
+
+// WHOLE: rows are whole chunks.  The loads of a part of a chunk, value by value,
+// take up to 32 registers, and rows in flight with them (8192 x 2048 bf16: gg
+// 50 -> 39 us; forward, with the parameters loaded once, 27 -> 14 us).  Measured:
+// 65536 x 4096 bf16 forward 211 us, backward 300 us, both at the 5.0 to 5.4 TB/s
+// of a large copy; 8192 x 384 fp32 forward 9.3, backward 9.9, gg 16.2 us (a copy
+// of as many bytes: 5, 8 and 13).
+//
+// Every kernel walks its rows with the next row's loads in flight while this
+// row is reduced and stored.  Rows past 2^31 - 1 do not exist, but row + stride
+// may pass that: 64-bit rows.
+template <typename T, int TPR, int NCH, int THREADS, bool WHOLE>
 __global__ __launch_bounds__(THREADS) void k_norm_fwd(NormArgs a) {
-  constexpr int V = kVec<T>;
-  __shared__ float lds[2 * 16];
-  const int row = blockIdx.x * (THREADS / TPR) + (int)threadIdx.x / TPR;
-  if (TPR == 64 && row >= a.N) return;
-  const T* x = (const T*)a.x + (int64_t)row * a.ldx;
-  T* y = (T*)a.y + (int64_t)row * a.ldy;
-  float v[NCH][V];
-  float s[1] = {0.f};
+  constexpr int V = kVec<T>, R = THREADS / TPR;
+  __shared__ float lds[2 * 2 * 16];
+  const int64_t stride = (int64_t)gridDim.x * R;
+  int64_t row = (int64_t)blockIdx.x * R + (int)threadIdx.x / TPR;
+  const float inv = 1.f / (float)a.D;
+  Raw<T> x[NCH];
+  load_row<T, TPR, NCH, WHOLE>(a.x, a.ldx, row, a, x);
+  float w[NCH][V], b[NCH][V];
 #pragma unroll
   for (int ch = 0; ch < NCH; ++ch) {
-    load_chunk<T>(x, chunk_col<T, TPR>(ch), a.D, v[ch]);
-#pragma unroll
-    for (int j = 0; j < V; ++j) s[0] += v[ch][j];
+    load_param<T, WHOLE>(a.w, a.wf32, chunk_col<T, TPR>(ch), a.D, 1.f, w[ch]);
+    load_param<T, WHOLE>(a.b, a.wf32, chunk_col<T, TPR>(ch), a.D, 0.f, b[ch]);
   }
-  row_sums<TPR, 1>(s, lds);
-  const float inv = 1.f / (float)a.D, mu = s[0] * inv;
-  float q[1] = {0.f};
+  for (int turn = 0; row < a.N; row += stride, turn ^= 1) {
+    float v[NCH][V], s[1] = {0.f};
 #pragma unroll
-  for (int ch = 0; ch < NCH; ++ch) {
-    const int c0 = chunk_col<T, TPR>(ch);
+    for (int ch = 0; ch < NCH; ++ch)
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      v[ch][j] -= mu;
-      q[0] += c0 + j < a.D ? v[ch][j] * v[ch][j] : 0.f;
+      for (int j = 0; j < V; ++j) {
+        v[ch][j] = (float)x[ch].v[j];
+        s[0] += v[ch][j];
+      }
+    load_row<T, TPR, NCH, WHOLE>(a.x, a.ldx, row + stride, a, x);
+    row_sums<TPR, 1>(s, lds, turn);
+    const float mu = s[0] * inv;
+    float q[1] = {0.f};
+#pragma unroll
+    for (int ch = 0; ch < NCH; ++ch) {
+      const int c0 = chunk_col<T, TPR>(ch);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        v[ch][j] -= mu;
+        q[0] += c0 + j < a.D ? v[ch][j] * v[ch][j] : 0.f;
+      }
     }
-  }
-  row_sums<TPR, 1>(q, lds);
-  const float r = 1.f / sqrtf(q[0] * inv + a.eps);
-  if (a.mean && threadIdx.x % TPR == 0) {
-    a.mean[row] = mu;
-    a.rstd[row] = r;
-  }
+    row_sums<TPR, 1>(q, lds + 32, turn);
+    const float r = 1.f / sqrtf(q[0] * inv + a.eps);
+    if (a.mean && threadIdx.x % TPR == 0) {
+      a.mean[row] = mu;
+      a.rstd[row] = r;
+    }
 #pragma unroll
-  for (int ch = 0; ch < NCH; ++ch) {
-    const int c0 = chunk_col<T, TPR>(ch);
-    if (c0 >= a.D) break;
-    float w[V], b[V];
-    load_param<T>(a.w, a.wf32, c0, a.D, 1.f, w);
-    load_param<T>(a.b, a.wf32, c0, a.D, 0.f, b);
+    for (int ch = 0; ch < NCH; ++ch) {
+      const int c0 = chunk_col<T, TPR>(ch);
+      if (c0 >= a.D) break;
+      float y[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) w[j] = v[ch][j] * r * w[j] + b[j];
-    store_chunk<T>(y, c0, a.D, w);
+      for (int j = 0; j < V; ++j) y[j] = v[ch][j] * r * w[ch][j] + b[ch][j];
+      store_chunk<T, WHOLE>((T*)a.y + row * a.ldy, c0, a.D, y);
+    }
   }
 }
 
 // The column sums of a workgroup's rows to part[group][k][D].  With TPR = 64
 // the waves hold sums of the same columns: added through LDS in wave order.
-template <typename T, int TPR, int NCH, int THREADS, int NSUM>
+template <typename T, int TPR, int NCH, int THREADS, bool WHOLE, int NSUM>
 __device__ __forceinline__ void store_sums(const NormArgs& a, float (*acc)[NCH][kVec<T>], float* lds) {
   constexpr int V = kVec<T>, W = THREADS / TPR, COLS = 64 * V;
   float* part = a.part + (int64_t)blockIdx.x * NSUM * a.D;
@@ -177,8 +221,8 @@ __device__ __forceinline__ void store_sums(const NormArgs& a, float (*acc)[NCH][
     for (int ch = 0; ch < NCH; ++ch) {
       const int c0 = chunk_col<T, TPR>(ch);
       if constexpr (TPR == THREADS) {
-        store_chunk<float>(part + (int64_t)k * a.D, c0, a.D, acc[k][ch]);
-        if constexpr (V == 8) store_chunk<float>(part + (int64_t)k * a.D, c0 + 4, a.D, acc[k][ch] + 4);
+        store_chunk<float, WHOLE>(part + (int64_t)k * a.D, c0, a.D, acc[k][ch]);
+        if constexpr (V == 8) store_chunk<float, WHOLE>(part + (int64_t)k * a.D, c0 + 4, a.D, acc[k][ch] + 4);
       } else {
         const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
         __syncthreads();
@@ -196,188 +240,209 @@ __device__ __forceinline__ void store_sums(const NormArgs& a, float (*acc)[NCH][
     }
 }
 
-template <typename T, int TPR, int NCH, int THREADS>
+template <typename T, int TPR, int NCH, int THREADS, bool WHOLE>
 __global__ __launch_bounds__(THREADS) void k_norm_bwd(NormArgs a) {
   constexpr int V = kVec<T>, R = THREADS / TPR;
-  __shared__ float lds[TPR == THREADS ? 64 : R * 64 * V];
+  __shared__ float lds[TPR == THREADS ? 2 * 2 * 16 : R * 64 * V];
   float w[NCH][V], acc[2][NCH][V];
 #pragma unroll
   for (int ch = 0; ch < NCH; ++ch) {
-    load_param<T>(a.w, a.wf32, chunk_col<T, TPR>(ch), a.D, 1.f, w[ch]);
+    load_param<T, WHOLE>(a.w, a.wf32, chunk_col<T, TPR>(ch), a.D, 1.f, w[ch]);
 #pragma unroll
     for (int j = 0; j < V; ++j) acc[0][ch][j] = acc[1][ch][j] = 0.f;
   }
   const float inv = 1.f / (float)a.D;
-  for (int row = blockIdx.x * R + (int)threadIdx.x / TPR; row < a.N; row += gridDim.x * R) {
-    const T* x = (const T*)a.x + (int64_t)row * a.ldx;
-    const T* dy = (const T*)a.dy + (int64_t)row * a.lddy;
-    const float mu = a.mean[row], r = a.rstd[row];
+  const int64_t stride = (int64_t)gridDim.x * R;
+  int64_t row = (int64_t)blockIdx.x * R + (int)threadIdx.x / TPR;
+  Raw<T> x[NCH], dy[NCH];
+  load_row<T, TPR, NCH, WHOLE>(a.x, a.ldx, row, a, x);
+  load_row<T, TPR, NCH, WHOLE>(a.dy, a.lddy, row, a, dy);
+  for (int turn = 0; row < a.N; row += stride, turn ^= 1) {
+    const float r = a.rstd[row], mr = -a.mean[row] * r;
     float xh[NCH][V], g[NCH][V], s[2] = {0.f, 0.f};
+    // past D: dy reads 0 there, and so nothing of xh counts
 #pragma unroll
-    for (int ch = 0; ch < NCH; ++ch) {
-      const int c0 = chunk_col<T, TPR>(ch);
-      load_chunk<T>(x, c0, a.D, xh[ch]);
-      load_chunk<T>(dy, c0, a.D, g[ch]);
+    for (int ch = 0; ch < NCH; ++ch)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        xh[ch][j] = (xh[ch][j] - mu) * r;  // past D: dy reads 0 there
+        xh[ch][j] = (float)x[ch].v[j] * r + mr;
+        g[ch][j] = (float)dy[ch].v[j];
         acc[0][ch][j] += g[ch][j] * xh[ch][j];
         acc[1][ch][j] += g[ch][j];
         g[ch][j] *= w[ch][j];
         s[0] += g[ch][j];
         s[1] += g[ch][j] * xh[ch][j];
       }
-    }
-    if (!a.y) continue;
-    row_sums<TPR, 2>(s, lds);
-    const float m1 = s[0] * inv, m2 = s[1] * inv;
-    T* dx = (T*)a.y + (int64_t)row * a.ldy;
+    load_row<T, TPR, NCH, WHOLE>(a.x, a.ldx, row + stride, a, x);
+    load_row<T, TPR, NCH, WHOLE>(a.dy, a.lddy, row + stride, a, dy);
+    if (!a.y) continue;  // uniform
+    row_sums<TPR, 2>(s, lds, turn);
+    const float m1 = -r * s[0] * inv, m2 = -r * s[1] * inv;
 #pragma unroll
     for (int ch = 0; ch < NCH; ++ch) {
       const int c0 = chunk_col<T, TPR>(ch);
       if (c0 >= a.D) break;
 #pragma unroll
-      for (int j = 0; j < V; ++j) g[ch][j] = r * (g[ch][j] - m1 - xh[ch][j] * m2);
-      store_chunk<T>(dx, c0, a.D, g[ch]);
+      for (int j = 0; j < V; ++j) g[ch][j] = r * g[ch][j] + (m1 + xh[ch][j] * m2);
+      store_chunk<T, WHOLE>((T*)a.y + row * a.ldy, c0, a.D, g[ch]);
     }
   }
-  if (a.part) store_sums<T, TPR, NCH, THREADS, 2>(a, acc, lds);
+  if (a.part) store_sums<T, TPR, NCH, THREADS, WHOLE, 2>(a, acc, lds);
 }
 
-template <typename T, int TPR, int NCH, int THREADS>
+// The sums of t = cw dy - r (a mean(g xh) + g mean(a xh)) and of a P(g) follow
+// from seven sums over the row itself, taken at once:
+//   sum t      = sum(cw dy)    - r (mean(g xh) sum a      + mean(a xh) sum g)
+//   sum t xh   = sum(cw dy xh) - r (mean(g xh) sum(a xh) + mean(a xh) sum(g xh))
+//   sum a P(g) = sum a g - mean(g) sum a - mean(g xh) sum(a xh)
+// so there is one reduction, and about 25 operations per element (they are
+// what bounds this kernel where its rows come from the cache).
+template <typename T, int TPR, int NCH, int THREADS, bool WHOLE>
 __global__ __launch_bounds__(THREADS) void k_norm_gg(NormArgs a) {
   constexpr int V = kVec<T>, R = THREADS / TPR;
-  __shared__ float lds[TPR == THREADS ? 64 : R * 64 * V];
-  float w[NCH][V], acc[1][NCH][V];
+  __shared__ float lds[TPR == THREADS ? 2 * 7 * 16 : R * 64 * V];
+  float w[NCH][V], cw[NCH][V], acc[1][NCH][V];
 #pragma unroll
   for (int ch = 0; ch < NCH; ++ch) {
-    load_param<T>(a.w, a.wf32, chunk_col<T, TPR>(ch), a.D, 1.f, w[ch]);
+    load_param<T, WHOLE>(a.w, a.wf32, chunk_col<T, TPR>(ch), a.D, 1.f, w[ch]);
+    load_param<T, WHOLE>(a.cw, a.wf32, chunk_col<T, TPR>(ch), a.D, 0.f, cw[ch]);
 #pragma unroll
     for (int j = 0; j < V; ++j) acc[0][ch][j] = 0.f;
   }
   const float inv = 1.f / (float)a.D;
-  for (int row = blockIdx.x * R + (int)threadIdx.x / TPR; row < a.N; row += gridDim.x * R) {
-    const T* x = (const T*)a.x + (int64_t)row * a.ldx;
-    const T* dyp = (const T*)a.dy + (int64_t)row * a.lddy;
-    const float mu = a.mean[row], r = a.rstd[row];
-    float xh[NCH][V], dy[NCH][V], c[NCH][V], s[4] = {0.f, 0.f, 0.f, 0.f};
+  const int64_t stride = (int64_t)gridDim.x * R;
+  int64_t row = (int64_t)blockIdx.x * R + (int)threadIdx.x / TPR;
+  Raw<T> nx[NCH], ndy[NCH], na[NCH];
+  if (!a.a)
+#pragma unroll
+    for (int ch = 0; ch < NCH; ++ch)
+#pragma unroll
+      for (int j = 0; j < V; ++j) na[ch].v[j] = (T)0.f;
+  const auto fetch = [&](int64_t n) {
+    load_row<T, TPR, NCH, WHOLE>(a.x, a.ldx, n, a, nx);
+    load_row<T, TPR, NCH, WHOLE>(a.dy, a.lddy, n, a, ndy);
+    if (a.a) load_row<T, TPR, NCH, WHOLE>(a.a, a.lda, n, a, na);
+  };
+  fetch(row);
+  for (int turn = 0; row < a.N; row += stride, turn ^= 1) {
+    const float r = a.rstd[row], mr = -a.mean[row] * r;
+    Raw<T> x[NCH], dy[NCH], c[NCH];
+    float s[7] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    // past D: dy and a read 0 there, and so nothing of xh counts
 #pragma unroll
     for (int ch = 0; ch < NCH; ++ch) {
-      const int c0 = chunk_col<T, TPR>(ch);
-      load_chunk<T>(x, c0, a.D, xh[ch]);
-      load_chunk<T>(dyp, c0, a.D, dy[ch]);
-      if (a.a) {
-        load_chunk<T>((const T*)a.a + (int64_t)row * a.lda, c0, a.D, c[ch]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) c[ch][j] = 0.f;
-      }
+      x[ch] = nx[ch];
+      dy[ch] = ndy[ch];
+      c[ch] = na[ch];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        xh[ch][j] = c0 + j < a.D ? (xh[ch][j] - mu) * r : 0.f;
-        const float g = dy[ch][j] * w[ch][j];
+        const float xh = (float)x[ch].v[j] * r + mr, d = (float)dy[ch].v[j], ca = (float)c[ch].v[j];
+        const float g = d * w[ch][j], cd = d * cw[ch][j];
         s[0] += g;
-        s[1] += g * xh[ch][j];
-        s[2] += c[ch][j];
-        s[3] += c[ch][j] * xh[ch][j];
+        s[1] += g * xh;
+        s[2] += ca;
+        s[3] += ca * xh;
+        s[4] += cd;
+        s[5] += cd * xh;
+        s[6] += ca * g;
       }
     }
-    row_sums<TPR, 4>(s, lds);
+    fetch(row + stride);
+    row_sums<TPR, 7>(s, lds, turn);
     const float mg = s[0] * inv, mgx = s[1] * inv, ma = s[2] * inv, max_ = s[3] * inv;
-    // second round: mean(t), mean(t xh), mean(a P(g)); gdy goes out on the way
-    float u[3] = {0.f, 0.f, 0.f};
+    const float mt = s[4] * inv - r * (mgx * ma + max_ * mg);
+    const float mtx = s[5] * inv - r * (2.f * mgx * max_);
+    const float map = s[6] * inv - mg * ma - mgx * max_;
+    // P(a) r = pa0 + r a + pa1 xh;  gx = o0 + o1 xh + o2 a + o3 g + r cw dy
+    const float pa0 = -r * ma, pa1 = -r * max_;
+    const float o0 = -r * mt, o1 = -(r * mtx + r * r * map), o2 = -r * r * mgx, o3 = -r * r * max_;
 #pragma unroll
     for (int ch = 0; ch < NCH; ++ch) {
       const int c0 = chunk_col<T, TPR>(ch);
-      float cw[V], cb[V], gdy[V];
-      load_param<T>(a.cw, a.wf32, c0, a.D, 0.f, cw);
-      load_param<T>(a.cb, a.wf32, c0, a.D, 0.f, cb);
+      float gdy[V], gx[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const bool in = c0 + j < a.D;
-        const float g = dy[ch][j] * w[ch][j];
-        const float ca = c[ch][j];
-        const float pa = in ? ca - ma - xh[ch][j] * max_ : 0.f;
-        const float pg = g - mg - xh[ch][j] * mgx;
-        acc[0][ch][j] += dy[ch][j] * r * pa;
-        gdy[j] = w[ch][j] * r * pa + cw[j] * xh[ch][j] + cb[j];
-        const float t = cw[j] * dy[ch][j] - r * (ca * mgx + g * max_);
-        c[ch][j] = t;
-        u[0] += t;
-        u[1] += t * xh[ch][j];
-        u[2] += in ? (ca - ma) * pg : 0.f;  // mean(pg) is 0: a without its own mean
+        const float xh = (float)x[ch].v[j] * r + mr, d = (float)dy[ch].v[j], ca = (float)c[ch].v[j];
+        const float pa = ca * r + (xh * pa1 + pa0);
+        acc[0][ch][j] += d * pa;
+        gdy[j] = w[ch][j] * pa + cw[ch][j] * xh;
+        gx[j] = (o0 + o1 * xh) + o2 * ca + d * (o3 * w[ch][j] + r * cw[ch][j]);
       }
-      if (a.gx && c0 < a.D) store_chunk<T>((T*)a.gx + (int64_t)row * a.ldgx, c0, a.D, gdy);
-    }
-    if (!a.y) continue;
-    row_sums<TPR, 3>(u, lds);
-    const float mt = u[0] * inv, mtx = r * (u[1] * inv) + r * r * (u[2] * inv);
-#pragma unroll
-    for (int ch = 0; ch < NCH; ++ch) {
-      const int c0 = chunk_col<T, TPR>(ch);
       if (c0 >= a.D) break;
-      float o[V];
+      if (a.gx) {
+        if (a.cb) {
+          float cb[V];
+          load_param<T, WHOLE>(a.cb, a.wf32, c0, a.D, 0.f, cb);
 #pragma unroll
-      for (int j = 0; j < V; ++j) o[j] = r * (c[ch][j] - mt) - xh[ch][j] * mtx;
-      store_chunk<T>((T*)a.y + (int64_t)row * a.ldy, c0, a.D, o);
+          for (int j = 0; j < V; ++j) gdy[j] += cb[j];
+        }
+        store_chunk<T, WHOLE>((T*)a.gx + row * a.ldgx, c0, a.D, gdy);
+      }
+      if (a.y) store_chunk<T, WHOLE>((T*)a.y + row * a.ldy, c0, a.D, gx);
     }
   }
-  if (a.part) store_sums<T, TPR, NCH, THREADS, 1>(a, acc, lds);
+  if (a.part) store_sums<T, TPR, NCH, THREADS, WHOLE, 1>(a, acc, lds);
 }
 
 // out_k[col] = sum over groups of part[group][k][col], in group order within
-// each of 32 lanes' strides, the strides in lane order.
+// each of 64 lanes' strides, the strides in lane order.
 template <typename TP>
 __global__ __launch_bounds__(1024) void k_norm_sums(const float* part, int groups, int nsum, int D, void* o0,
                                                     void* o1) {
-  __shared__ float lds[32][33];
-  const int c = threadIdx.x & 31, s = threadIdx.x >> 5, k = blockIdx.y;
-  const int col = blockIdx.x * 32 + c;
+  __shared__ float lds[64][17];
+  const int c = threadIdx.x & 15, s = threadIdx.x >> 4, k = blockIdx.y;
+  const int col = blockIdx.x * 16 + c;
   float t = 0.f;
   if (col < D) {
 #pragma unroll 8
-    for (int g = s; g < groups; g += 32) t += part[((int64_t)g * nsum + k) * D + col];
+    for (int g = s; g < groups; g += 64) t += part[((int64_t)g * nsum + k) * D + col];
   }
   lds[s][c] = t;
   __syncthreads();
   if (s == 0 && col < D) {
     float v = 0.f;
-    for (int i = 0; i < 32; ++i) v += lds[i][c];
+#pragma unroll 16
+    for (int i = 0; i < 64; ++i) v += lds[i][c];
     TP* o = (TP*)(k == 0 ? o0 : o1);
     if (o) o[col] = (TP)v;
   }
 }
 
-// Rows walked by one workgroup at least, where column sums are formed: their
-// partial sums are [groups][2][D] fp32, written and read once.
-constexpr int kNormGroups = 1024;
-
 struct Shape {
-  int tpr, nch, threads;
+  int tpr, nch, threads;  // threads of a row, chunks of each, threads of a workgroup
+  int per() const { return threads / tpr; }
 };
 
-// The narrowest row layout that holds D values in registers.
+// One chunk a thread as long as a workgroup can hold the row that way: the
+// fewest registers, so the most rows in flight (backward of 65536 x 4096 bf16:
+// 453 us with 256 threads of two chunks, 313 with 512 of one).  A row in more
+// than one wave is a workgroup's: its barriers must be met by all.
 template <typename T>
 Shape norm_shape(int64_t D) {
   const int64_t c = (D + kVec<T> - 1) / kVec<T>;  // chunks of a row
   if (c <= 64) return {64, 1, 256};
-  if (c <= 128) return {64, 2, 256};
+  if (c <= 128) return {128, 1, 128};
   if (c <= 256) return {256, 1, 256};
-  if (c <= 512) return {256, 2, 256};
+  if (c <= 512) return {512, 1, 512};
   if (c <= 1024) return {1024, 1, 1024};
   if (c <= 2048) return {1024, 2, 1024};
   return {1024, 4, 1024};
 }
 
-#define NORM_DISPATCH(KERNEL, T, sh, grid, st, args)                                                  \
-  do {                                                                                                \
-    if (sh.tpr == 64 && sh.nch == 1) KERNEL<T, 64, 1, 256><<<grid, 256, 0, st>>>(args);               \
-    else if (sh.tpr == 64) KERNEL<T, 64, 2, 256><<<grid, 256, 0, st>>>(args);                         \
-    else if (sh.tpr == 256 && sh.nch == 1) KERNEL<T, 256, 1, 256><<<grid, 256, 0, st>>>(args);        \
-    else if (sh.tpr == 256) KERNEL<T, 256, 2, 256><<<grid, 256, 0, st>>>(args);                       \
-    else if (sh.nch == 1) KERNEL<T, 1024, 1, 1024><<<grid, 1024, 0, st>>>(args);                      \
-    else if (sh.nch == 2) KERNEL<T, 1024, 2, 1024><<<grid, 1024, 0, st>>>(args);                      \
-    else KERNEL<T, 1024, 4, 1024><<<grid, 1024, 0, st>>>(args);                                       \
+#define NORM_SHAPES(KERNEL, T, WHOLE, sh, grid, st, args)                                                \
+  do {                                                                                                   \
+    if (sh.tpr == 64) KERNEL<T, 64, 1, 256, WHOLE><<<grid, 256, 0, st>>>(args);                          \
+    else if (sh.tpr == 128) KERNEL<T, 128, 1, 128, WHOLE><<<grid, 128, 0, st>>>(args);                   \
+    else if (sh.tpr == 256) KERNEL<T, 256, 1, 256, WHOLE><<<grid, 256, 0, st>>>(args);                   \
+    else if (sh.tpr == 512) KERNEL<T, 512, 1, 512, WHOLE><<<grid, 512, 0, st>>>(args);                   \
+    else if (sh.nch == 1) KERNEL<T, 1024, 1, 1024, WHOLE><<<grid, 1024, 0, st>>>(args);                  \
+    else if (sh.nch == 2) KERNEL<T, 1024, 2, 1024, WHOLE><<<grid, 1024, 0, st>>>(args);                  \
+    else KERNEL<T, 1024, 4, 1024, WHOLE><<<grid, 1024, 0, st>>>(args);                                   \
+  } while (0)
+#define NORM_DISPATCH(KERNEL, T, sh, grid, st, args)                          \
+  do {                                                                        \
+    if (args.D % kVec<T> == 0) NORM_SHAPES(KERNEL, T, true, sh, grid, st, args); \
+    else NORM_SHAPES(KERNEL, T, false, sh, grid, st, args);                   \
   } while (0)
 
 #define NORM_TYPES(dtype, ...)                                     \
@@ -387,10 +452,15 @@ Shape norm_shape(int64_t D) {
     else { typedef float T; __VA_ARGS__; }                         \
   } while (0)
 
-int groups_of(const ttt_norm_problem* p, const Shape& sh) {
-  const int64_t per = sh.threads / sh.tpr, n = (p->rows + per - 1) / per;
-  return (int)(n < kNormGroups ? n : kNormGroups);
+// Workgroups of a launch at most, in threads: eight of 256 per CU; half as
+// many where column sums are formed, each of which is written and read once.
+constexpr int64_t kFwdThreads = 2048 * 256, kSumThreads = 1024 * 256;
+
+int walkers(const ttt_norm_problem* p, const Shape& sh, int64_t threads) {
+  const int64_t n = (p->rows + sh.per() - 1) / sh.per(), most = threads / sh.threads;
+  return (int)(n < most ? n : most);
 }
+int groups_of(const ttt_norm_problem* p, const Shape& sh) { return walkers(p, sh, kSumThreads); }
 
 Shape shape_of(const ttt_norm_problem* p) {
   return p->dtype == TTT_F32 ? norm_shape<float>(p->cols) : norm_shape<_Float16>(p->cols);
@@ -437,7 +507,7 @@ int finish(const char* what) {
 
 void launch_sums(const ttt_norm_problem* p, const float* part, int groups, int nsum, void* o0, void* o1,
                  hipStream_t st) {
-  const dim3 grid((unsigned)((p->cols + 31) / 32), nsum);
+  const dim3 grid((unsigned)((p->cols + 15) / 16), nsum);
   NORM_TYPES(p->param_dtype, (k_norm_sums<T><<<grid, 1024, 0, st>>>(part, groups, nsum, (int)p->cols, o0, o1)));
 }
 
@@ -473,8 +543,7 @@ int ttt_norm_fwd(const ttt_norm_problem* p, const ttt_rows* x, const void* weigh
   a.wf32 = p->param_dtype == TTT_F32;
   a.eps = p->eps;
   const Shape sh = shape_of(p);
-  const int per = sh.threads / sh.tpr;
-  const unsigned grid = (unsigned)((p->rows + per - 1) / per);
+  const unsigned grid = (unsigned)walkers(p, sh, kFwdThreads);
   const hipStream_t st = (hipStream_t)stream;
   NORM_TYPES(p->dtype, NORM_DISPATCH(k_norm_fwd, T, sh, grid, st, a));
   return finish("ttt_norm_fwd");
