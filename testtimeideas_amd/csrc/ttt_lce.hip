@@ -61,49 +61,50 @@ struct CopyArgs {
 };
 
 __global__ __launch_bounds__(256) void k_copy_rows(CopyArgs a) {
-  const int chunks = round8(a.C) / 8;
-  const int64_t total = (int64_t)a.R * chunks;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int r = (int)(i / chunks), c = 8 * (int)(i % chunks);
-    const uint16_t* s = (const uint16_t*)a.src + (int64_t)r * a.ld + c;
-    uint16_t v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (!a.live || a.live[r] != 0.f) {
+  const int row = blockIdx.x * 4 + (threadIdx.x >> 6);  // a wave a row
+  if (row >= a.R) return;
+  const uint16_t* s = (const uint16_t*)a.src + row * a.ld;
+  const int width = round8(a.C);
+  uint16_t* d = (uint16_t*)a.dst + (int64_t)row * width;
+  const bool live = !a.live || a.live[row] != 0.f;
+  for (int c = 8 * (threadIdx.x & 63); c < width; c += 512) {
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (live) {
       if (c + 8 <= a.C) {
-        __builtin_memcpy(v, s, 16);
+        __builtin_memcpy(&v, s + c, 16);
       } else {
-        for (int j = 0; c + j < a.C; ++j) v[j] = s[j];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j / 2] |= c + j < a.C ? (uint32_t)s[c + j] << (16 * (j & 1)) : 0u;
       }
     }
-    __builtin_memcpy((uint16_t*)a.dst + i * 8, v, 16);
+    *(u32x4*)(d + c) = v;
   }
 }
 
 // ---------------------------------------------------------------------------
-// The products' tile shapes.  16-bit: 256 x 256 (eight waves of 128 x 64) and
-// 128 x 128 (four of 64 x 64); two accumulators: 256 x 128 (eight of 64 x 64)
-// and 128 x 128.  fp32: 128 x 128 (eight of 64 x 32) and 64 x 128 (four of
-// 32 x 64).  Logits of few tokens or few tiles: 32 x 32 (DirectProduct).
+// The products' tile shapes.  16-bit: 256 x 256 (eight waves of 128 x 64), with
+// one accumulator, and 128 x 128 (four of 64 x 64).  fp32: 128 x 128 (eight of
+// 64 x 32) and 64 x 128 (four of 32 x 64).  Logits of few tokens or few tiles:
+// 32 x 32 (DirectProduct).
 // ---------------------------------------------------------------------------
 enum : int { kDirect = 0, kSmall = 1, kBig = 2 };
 
-template <typename T, bool MT, bool NT, bool DUAL, int SIZE>
+template <typename T, bool MT, bool NT, int SIZE>
 struct ProductOf {
   static constexpr bool big = SIZE == kBig;
-  static constexpr int BM = big ? 256 : 128, BN = big && !DUAL ? 256 : 128;
-  static constexpr int WM = DUAL && big ? 4 : 2, WN = DUAL && big ? 2 : big ? 4 : 2;
-  typedef TileProduct<T, BM, BN, WM, WN, MT, NT> type;
+  typedef TileProduct<T, big ? 256 : 128, big ? 256 : 128, 2, big ? 4 : 2, MT, NT> type;
 };
-template <bool MT, bool NT, bool DUAL, int SIZE>
-struct ProductOf<float, MT, NT, DUAL, SIZE> {
+template <bool MT, bool NT, int SIZE>
+struct ProductOf<float, MT, NT, SIZE> {
   static constexpr bool big = SIZE == kBig;
   typedef SplitProduct<big ? 128 : 64, 128, 2, big ? 4 : 2, MT, NT> type;
 };
-template <typename T, bool DUAL>
-struct ProductOf<T, false, false, DUAL, kDirect> {
+template <typename T>
+struct ProductOf<T, false, false, kDirect> {
   typedef DirectProduct<T> type;
 };
-template <bool DUAL>
-struct ProductOf<float, false, false, DUAL, kDirect> {
+template <>
+struct ProductOf<float, false, false, kDirect> {
   typedef DirectProduct<float> type;
 };
 
@@ -195,7 +196,7 @@ __device__ __forceinline__ void store_tile(const P& tp, char* lds, void* out, in
 template <typename T, int MODE, int SIZE>
 __global__ __launch_bounds__((kThreadsOf<T, SIZE>), 2) void k_logits(ZArgs a) {
   constexpr bool kDual = MODE >= kHSum;
-  typedef typename ProductOf<T, false, false, kDual, SIZE>::type P;
+  typedef typename ProductOf<T, false, false, SIZE>::type P;
   constexpr int MI = P::MI, NI = P::NI;
   const typename P::Lds lds = lds_of<T, P>();
   int tm, tn;
@@ -319,7 +320,7 @@ struct OutArgs {
 
 template <typename T, bool NT, int SIZE>
 __global__ __launch_bounds__((kThreadsOf<T, SIZE>), 2) void k_product(OutArgs a) {
-  typedef typename ProductOf<T, true, NT, false, SIZE>::type P;
+  typedef typename ProductOf<T, true, NT, SIZE>::type P;
   constexpr int MI = P::MI, NI = P::NI;
   const typename P::Lds lds = lds_of<T, P>();
   const int s = blockIdx.x / (a.tm * a.tn), id = blockIdx.x % (a.tm * a.tn);
@@ -381,6 +382,7 @@ __global__ __launch_bounds__(256) void k_finish(OutArgs a) {
   const float al = *a.alpha;
   const int cnt = total - i4 < 4 ? (int)(total - i4) : 4;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
   for (int s = 0; s < a.split; ++s) {
     const float* p = a.part + s * total + i4;
     if (cnt == 4) {
@@ -580,7 +582,7 @@ __global__ __launch_bounds__(1024) void k_factors(RowArgs a) {
     bm = block_max(bm, lds);
   }
   const int stride = gridDim.x * 1024;
-#pragma unroll 2
+#pragma unroll 4
   for (int n = blockIdx.x * 1024 + threadIdx.x; n < a.N; n += stride) {
     const float w = row_weight(a, n);
     const float up = a.grad_loss[a.reduction == TTT_REDUCE_NONE ? n : 0];
@@ -601,7 +603,7 @@ __global__ __launch_bounds__(1024) void k_factors(RowArgs a) {
   }
   top = fmaxf(block_max(top, lds), 1e-30f);
   const float s = (a.dtype == TTT_F16 ? kF16Scale : 1.f) / top;
-#pragma unroll 2
+#pragma unroll 4
   for (int n = threadIdx.x; n < a.N; n += 1024) a.colmul[n] = a.coef[n] * s;
   if (threadIdx.x == 0) *a.alpha = a.dtype == TTT_F16 ? top * (1.f / kF16Scale) : top;
 }
@@ -663,6 +665,7 @@ __global__ __launch_bounds__(256) void k_row_h(HArgs a) {
     if (a.b) {
       const float v = (float)((const T*)a.x)[n64 * a.ldx + i];
       float q = 0.f;
+#pragma unroll 4
       for (int k = 0; k < a.split; ++k) q += a.gb[((int64_t)k * a.N + n64) * a.d + i];
       const float bt = (float)((const T*)a.b)[t * a.ldb + i];
       if (sizeof(T) == 2) q += a.rest[n] * bt;
@@ -743,21 +746,24 @@ struct Spread {  // the tile shape of a product, and the workgroups of a tile
 
 // A tile's rows along m, and tokens (or rows) along n.
 int tile_m(const Plan& k, int size) { return size == kDirect ? 32 : k.f32 ? (size == kBig ? 128 : 64) : size == kBig ? 256 : 128; }
-int tile_n(const Plan& k, int size, bool dual) { return size == kDirect ? 32 : !k.f32 && size == kBig && !dual ? 256 : 128; }
+int tile_n(const Plan& k, int size) { return size == kDirect ? 32 : !k.f32 && size == kBig ? 256 : 128; }
 
 // The tile shape of the logits: large where such tiles fill the card, direct
-// for a few tokens or few tiles.
+// for a few tokens or few tiles.  Two accumulators of 16-bit types leave room
+// for 256 x 128 at most, and two workgroups of 128 x 128 on a CU, which do not
+// wait for each other, are faster (4096 x 1024 x 16384 bf16: 391 and 354 us).
 int logits_size(const Plan& k, bool dual, int M, int N) {
-  const auto tiles = [&](int size) { return cdiv(M, tile_m(k, size)) * cdiv(N, tile_n(k, size, dual)); };
+  const auto tiles = [&](int size) { return cdiv(M, tile_m(k, size)) * cdiv(N, tile_n(k, size)); };
   if (N <= 32 || tiles(kSmall) < 96) return kDirect;
+  if (dual && !k.f32) return kSmall;
   return tiles(kBig) >= (k.f32 ? 512 : 192) ? kBig : kSmall;
 }
 
-// Rows of parts that launch_logits writes for M vocabulary rows: one per wave
-// along them.
+// Rows of parts that launch_logits writes for M vocabulary rows: one for each
+// of the two waves that share a tile's.
 int parts_of(const Plan& k, bool dual, int M, int N) {
   const int size = logits_size(k, dual, M, N);
-  return (int)cdiv(M, tile_m(k, size)) * (dual && size == kBig && !k.f32 ? 4 : 2);
+  return (int)cdiv(M, tile_m(k, size)) * 2;
 }
 
 // The tile shape and split of a plain product of k in `segs` segments: the
@@ -770,10 +776,10 @@ Spread spread_of(const Plan& p, int M, int N, int64_t k, bool keep) {
   Spread best{kSmall, 1};
   double least = 1e30;
   for (int size = kSmall; size <= kBig; ++size) {
-    const int slots = p.f32 ? (size == kBig ? 512 : 1024) : size == kBig ? 256 : 512;
-    const double us = p.f32 ? (size == kBig ? 3.2 : 3.4) : size == kBig ? 1.8 : 1.6;
-    const int64_t tiles = cdiv(M, tile_m(p, size)) * cdiv(N, tile_n(p, size, false));
-    for (int split = 1; split <= kMaxSplit; split += split < 4 ? 1 : split < 16 ? 2 : 8) {
+    const int slots = size == kBig ? 256 : 512;
+    const double us = p.f32 ? (size == kBig ? 1.5 : 1.7) : size == kBig ? 1.75 : 1.25;
+    const int64_t tiles = cdiv(M, tile_m(p, size)) * cdiv(N, tile_n(p, size));
+    for (int split = 1; split <= kMaxSplit; split += split < 8 ? 1 : split < 24 ? 2 : 8) {
       if (split > 1 && split * 4 > steps) break;
       const int chunk = (int)cdiv(steps, split);
       const double rounds = (double)cdiv(tiles * split, slots);
@@ -874,9 +880,7 @@ void add_product(SegList* l, Operand m, Operand n, int k) {
 }
 
 void launch_copy(const void* src, int64_t ld, int R, int C, void* dst, const float* live, hipStream_t st) {
-  CopyArgs a{src, ld, R, C, dst, live};
-  const int64_t n = cdiv((int64_t)R * (round8(C) / 8), 256);
-  k_copy_rows<<<(unsigned)(n < 8192 ? n : 8192), 256, 0, st>>>(a);
+  k_copy_rows<<<(unsigned)cdiv(R, 4), 256, 0, st>>>(CopyArgs{src, ld, R, C, dst, live});
 }
 
 template <int MODE>
@@ -884,13 +888,21 @@ void launch_logits(const Plan& k, ZArgs a, hipStream_t st) {
   constexpr bool dual = MODE >= kHSum;
   const int size = logits_size(k, dual, a.M, a.N);
   a.tm = (int)cdiv(a.M, tile_m(k, size));
-  a.tn = (int)cdiv(a.N, tile_n(k, size, dual));
+  a.tn = (int)cdiv(a.N, tile_n(k, size));
   const unsigned grid = (unsigned)(a.tm * a.tn);
 #define LOGITS(T)                                                                     \
   do {                                                                                \
-    if (size == kBig) k_logits<T, MODE, kBig><<<grid, 512, 0, st>>>(a);               \
-    else if (size == kSmall) k_logits<T, MODE, kSmall><<<grid, 256, 0, st>>>(a);      \
-    else k_logits<T, MODE, kDirect><<<grid, 256, 0, st>>>(a);                         \
+    if (size == kDirect) {                                                            \
+      k_logits<T, MODE, kDirect><<<grid, 256, 0, st>>>(a);                            \
+      break;                                                                          \
+    }                                                                                 \
+    if constexpr (!dual || sizeof(T) == 4) {                                          \
+      if (size == kBig) {                                                             \
+        k_logits<T, MODE, kBig><<<grid, 512, 0, st>>>(a);                             \
+        break;                                                                        \
+      }                                                                               \
+    }                                                                                 \
+    k_logits<T, MODE, kSmall><<<grid, 256, 0, st>>>(a);                               \
   } while (0)
   if (k.dtype == TTT_F32) LOGITS(float);
   else if (k.dtype == TTT_BF16) LOGITS(__bf16);
@@ -928,7 +940,7 @@ void launch_product(const Plan& k, OutArgs a, bool nt, float* part, bool keep, c
   int steps = 0;
   for (int i = 0; i < a.l.n; ++i) steps += (int)cdiv(a.l.s[i].k, k.f32 ? 32 : 64);
   a.tm = (int)cdiv(a.M, tile_m(k, s.size));
-  a.tn = (int)cdiv(a.N, tile_n(k, s.size, false));
+  a.tn = (int)cdiv(a.N, tile_n(k, s.size));
   a.split = s.split;
   a.chunk = (int)cdiv(steps, s.split);
   a.part = keep || s.split > 1 ? part : nullptr;
