@@ -435,7 +435,7 @@ META_8K = dict(vocab_size=512, num_keys=64, max_seq_len=8192, context_len=6144, 
 META_8K_H100_S_PER_IT = 1.27
 
 
-def meta_bench(steps: int, warmup: int, dev) -> dict:
+def meta_bench(steps: int, warmup: int, dev, fused_tail: bool = False) -> dict:
     """Seconds per meta-training iteration of the reference TTT model at
     meta_8k_v2 on this GPU, timed as the reference's loop is
     (scripts/train_meta.py:133-160): synthetic batch, meta_step, backward of
@@ -447,7 +447,7 @@ def meta_bench(steps: int, warmup: int, dev) -> dict:
     model = TTTModel(ModelConfig(vocab_size=c["vocab_size"], max_seq_len=c["max_seq_len"],
                                  window_size=c["window_size"], d_model=c["d_model"], n_heads=c["n_heads"],
                                  n_layers=c["n_layers"], d_ff=c["d_ff"], suffix_layers=c["suffix_layers"],
-                                 dual_mlp=c["dual_mlp"])).to(dev)
+                                 dual_mlp=c["dual_mlp"], fused_tail=fused_tail)).to(dev)
     opt = torch.optim.AdamW(model.parameters(), lr=c["lr"], weight_decay=0.0)
     gen = torch.Generator().manual_seed(1337)
 
@@ -476,7 +476,8 @@ def meta_bench(steps: int, warmup: int, dev) -> dict:
             "inner_loss": round(float(inner), 4), "outer_loss": round(float(outer), 4),
             "reference_h100_s_per_it": META_8K_H100_S_PER_IT,
             "config": "meta_8k_v2: b8 T8192 d_model 384 6 heads 8 layers (2 suffix) window 512 chunks 1024, "
-                      "4 inner steps on mlp_fast, fp32, AdamW"}
+                      "4 inner steps on mlp_fast, fp32, AdamW"
+                      + (", layer norms and loss on the library's kernels" if fused_tail else "")}
 
 
 def copy_calibration(mb: int, reps: int = 5) -> None:
@@ -502,6 +503,8 @@ def main():
     ap.add_argument("--no-graph", action="store_true", help="skip the HIP-graph replay of the step")
     ap.add_argument("--autotune", action="store_true",
                     help="measured split per kernel family and shape (testtimeideas_amd.autotune), tuned in warmup")
+    ap.add_argument("--fused-tail", action="store_true",
+                    help="META_8K with the model's layer norms and loss on the library's kernels")
     ap.add_argument("--copy-mb", type=int, default=0,
                     help="also run a plain device copy of this many MiB (counter calibration for rocprof)")
     args = ap.parse_args()
@@ -521,7 +524,7 @@ def main():
         copy_calibration(args.copy_mb)
     if args.config == "META_8K":
         torch.autograd.set_multithreading_enabled(False)
-        r = meta_bench(args.steps, args.warmup, dev)
+        r = meta_bench(args.steps, args.warmup, dev, args.fused_tail)
         print(json.dumps({"metric": "meta-train s/it (reference TTT model, meta_8k_v2)", "value": r["s_per_it"],
                           "unit": "s/it", "n_gpus": 1, "steps": args.steps, "warmup": args.warmup,
                           "ms_per_step": round(r["s_per_it"] * 1e3, 2), "higher_is_better": False,

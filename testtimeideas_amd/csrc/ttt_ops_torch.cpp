@@ -11,6 +11,8 @@
 #include <torch/extension.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
@@ -99,6 +101,23 @@ variable_list once(variable_list out, const variable_list& from) {
   for (Tensor& t : out)
     if (t.defined()) t = Once::apply(t, f[0], f[1], f[2], f[3], f[4], f[5]);
   return out;
+}
+
+// Refuses a backward pass that is being captured while an eager graph of one of
+// its leaves is alive.  The leaf's gradient node is then of the eager graph's
+// stream; the engine makes that stream wait for the captured one, the capture
+// ends with work that never joins it, and the process with it.
+void check_capture(std::initializer_list<Tensor> leaves) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  for (const Tensor& t : leaves) {
+    if (!t.defined() || !t.is_leaf() || !t.requires_grad()) continue;
+    const std::shared_ptr<torch::autograd::Node> node = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (!node) continue;
+    const auto stream = node->stream();
+    TORCH_CHECK(!stream || *stream == c10::impl::VirtualGuardImpl(t.device().type()).getStream(t.device()),
+                "a backward pass cannot be captured while a graph of the same leaf tensor, recorded on another "
+                "stream, is alive: drop that graph (the tensors computed from the leaf) before the capture");
+  }
 }
 
 Tensor as_type(const Tensor& t, const Tensor& like) {
@@ -202,6 +221,7 @@ struct NormBwd : public torch::autograd::Function<NormBwd> {
         if (have >> i & 1) c[i] = g[n++];
       if (!c[0].defined() && !c[1].defined() && !c[2].defined()) return out;
       const Launch on(s[1]);
+      check_capture({s[0], s[1], s[2]});
       const Tensor x = as_rows(s[1], false), dy = as_rows(s[0], false), w = packed(s[2]);
       Tensor a;
       if (c[0].defined()) a = as_rows(as_type(c[0], x), false);
@@ -258,6 +278,7 @@ struct Norm : public torch::autograd::Function<Norm> {
                nb = (given & 2) && ctx->needs_input_grad(2);
     variable_list out(4);
     if (!nx && !nw && !nb) return out;
+    check_capture({s[0], s[1]});
     const Tensor dy = as_type(g[0], s[0]);
     variable_list r;
     if (at::GradMode::is_enabled()) {
@@ -385,6 +406,7 @@ struct LceBwd : public torch::autograd::Function<LceBwd> {
       Tensor a = nx ? g[0] : Tensor(), b = nw ? g[nx ? 1 : 0] : Tensor();
       if (!a.defined() && !b.defined()) return out;
       const Launch on(s[1]);
+      check_capture({s[0], s[1], s[2]});
       const Tensor x = lce_rows(s[1]), w = lce_rows(s[2]);
       if (a.defined()) a = lce_rows(as_type(a, x));
       if (b.defined()) b = lce_rows(as_type(b, x));
@@ -436,6 +458,7 @@ struct Lce : public torch::autograd::Function<Lce> {
     const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1);
     variable_list out(6);
     if (!nx && !nw) return out;
+    check_capture({s[0], s[1]});
     Tensor go = g[0];
     if (go.scalar_type() != at::kFloat) go = go.to(at::kFloat);
     go = go.contiguous();

@@ -71,18 +71,27 @@ def _suffix_logits(model, params: Params, hidden: torch.Tensor) -> torch.Tensor:
     return functional_call(model, params, (None,), {"mode": "suffix", "prefix_hidden": hidden})
 
 
+def model_loss(model, params: Params, targets, mask, *, prefix_hidden=None, input_ids=None) -> torch.Tensor:
+    """The masked token loss of the suffix on prefix_hidden, or of the full
+    model on input_ids.  A model with ``fused_tail`` forms it without logits."""
+    if prefix_hidden is not None:
+        args, kwargs = (None,), {"mode": "suffix", "prefix_hidden": prefix_hidden}
+    elif input_ids is not None:
+        args, kwargs = (input_ids,), {"mode": "full"}
+    else:
+        raise ValueError("a loss needs prefix_hidden or input_ids")
+    cfg = getattr(model, "cfg", None)
+    if getattr(cfg, "fused_tail", False):
+        return functional_call(model, params, args, {**kwargs, "targets": targets, "mask": mask})
+    return token_loss(functional_call(model, params, args, kwargs), targets, mask)
+
+
 def inner_update(model, params: Params, trainable: List[str], targets, mask, lr: float, create_graph: bool, *,
                  prefix_hidden=None, input_ids=None) -> Tuple[Params, torch.Tensor]:
     """One SGD step of the trainable parameters on the suffix loss of
     prefix_hidden (or the full model's loss of input_ids); returns the new
     parameter dict and the loss before the step."""
-    if prefix_hidden is not None:
-        logits = _suffix_logits(model, params, prefix_hidden)
-    elif input_ids is not None:
-        logits = functional_call(model, params, (input_ids,), {"mode": "full"})
-    else:
-        raise ValueError("inner_update needs prefix_hidden or input_ids")
-    loss = token_loss(logits, targets, mask)
+    loss = model_loss(model, params, targets, mask, prefix_hidden=prefix_hidden, input_ids=input_ids)
     grads = torch.autograd.grad(loss, [params[n] for n in trainable], create_graph=create_graph,
                                 retain_graph=create_graph)
     stepped = dict(params)
@@ -116,8 +125,8 @@ def outer_loss(model, params: Params, hidden, targets, outer_mask, *, chunk_size
     for (s0, s1), n in zip(spans, counts):
         if n <= 0:
             continue
-        logits = _suffix_logits(model, params, hidden[:, s0:s1])
-        total = total + token_loss(logits, targets[:, s0:s1], outer_mask[:, s0:s1]) * n
+        loss = model_loss(model, params, targets[:, s0:s1], outer_mask[:, s0:s1], prefix_hidden=hidden[:, s0:s1])
+        total = total + loss * n
         n_all += n
     return total / max(n_all, 1.0)
 

@@ -14,6 +14,10 @@ windowed self-attention (``WindowedSelfAttention`` on the HIP kernels) and a
 GELU feed-forward; the blocks the inner loop adapts (the last
 ``suffix_layers``) sum a fast and, optionally, a slow feed-forward; a final
 LayerNorm and an untied output projection.
+
+With ``fused_tail`` the layer norms are the library's (``layer_norm``, same
+parameters), and a forward that is given targets returns their loss from the
+library's ``linear_cross_entropy`` instead of logits, which then never exist.
 """
 from __future__ import annotations
 
@@ -24,6 +28,8 @@ import torch
 from torch import nn
 
 from testtimeideas_amd.ttt_e2e.attention import WindowedSelfAttention
+from testtimeideas_amd.ttt_e2e.loss import linear_cross_entropy
+from testtimeideas_amd.ttt_e2e.norm import LayerNorm
 
 
 @dataclasses.dataclass
@@ -39,6 +45,11 @@ class ModelConfig:
     use_gradgrad_attention: bool = True
     suffix_layers: int = -1  # adapted blocks at the end; out of range (e.g. -1): every block
     dual_mlp: bool = True    # adapted blocks add a slow feed-forward to the fast one
+    fused_tail: bool = False  # layer norms and the head's loss on the library's kernels
+
+
+def _norm(cfg: ModelConfig) -> nn.LayerNorm:
+    return (LayerNorm if cfg.fused_tail else nn.LayerNorm)(cfg.d_model)
 
 
 class FeedForward(nn.Sequential):
@@ -55,10 +66,10 @@ class Block(nn.Module):
 
     def __init__(self, cfg: ModelConfig, adapted: bool):
         super().__init__()
-        self.ln1 = nn.LayerNorm(cfg.d_model)
+        self.ln1 = _norm(cfg)
         self.attn = WindowedSelfAttention(cfg.d_model, cfg.n_heads, cfg.window_size,
                                           use_gradgrad=cfg.use_gradgrad_attention)
-        self.ln2 = nn.LayerNorm(cfg.d_model)
+        self.ln2 = _norm(cfg)
         if adapted:
             self.ff_names = ("mlp_fast", "mlp_slow") if cfg.dual_mlp else ("mlp_fast",)
         else:
@@ -86,7 +97,7 @@ class TTTModel(nn.Module):
         self.prefix_layers = cfg.n_layers - n_adapted
         self.prefix_blocks = nn.ModuleList([Block(cfg, adapted=False) for _ in range(self.prefix_layers)])
         self.suffix_blocks = nn.ModuleList([Block(cfg, adapted=True) for _ in range(n_adapted)])
-        self.ln_f = nn.LayerNorm(cfg.d_model)
+        self.ln_f = _norm(cfg)
         self.head = nn.Linear(cfg.d_model, cfg.vocab_size, bias=False)
 
     def prefix_forward(self, input_ids: torch.Tensor) -> torch.Tensor:
@@ -96,21 +107,32 @@ class TTTModel(nn.Module):
             x = block(x)
         return x
 
-    def suffix_forward(self, hidden: torch.Tensor) -> torch.Tensor:
-        """Logits, [B, T, vocab], from hidden states after the prefix."""
+    def suffix_forward(self, hidden: torch.Tensor, targets: Optional[torch.Tensor] = None,
+                       mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Logits, [B, T, vocab], from hidden states after the prefix; or, with
+        targets (``fused_tail``), the mean loss over the positions where mask
+        is nonzero (all without one)."""
         for block in self.suffix_blocks:
             hidden = block(hidden)
-        return self.head(self.ln_f(hidden))
+        hidden = self.ln_f(hidden)
+        if targets is None:
+            return self.head(hidden)
+        return linear_cross_entropy(hidden, self.head.weight, targets, mask)
 
     def forward(self, input_ids: Optional[torch.Tensor] = None, *, mode: str = "full",
-                prefix_hidden: Optional[torch.Tensor] = None) -> torch.Tensor:
+                prefix_hidden: Optional[torch.Tensor] = None, targets: Optional[torch.Tensor] = None,
+                mask: Optional[torch.Tensor] = None) -> torch.Tensor:
         """mode "prefix": hidden states of input_ids; "suffix": logits from
-        prefix_hidden; anything else ("full"): logits of input_ids."""
+        prefix_hidden; anything else ("full"): logits of input_ids.  With
+        targets (``fused_tail`` only; not in mode "prefix"), their loss in
+        place of the logits."""
+        if targets is not None and (mode == "prefix" or not self.cfg.fused_tail):
+            raise ValueError("targets need fused_tail and a mode that ends in logits")
         if mode == "suffix":
             if prefix_hidden is None:
                 raise ValueError("mode='suffix' starts from prefix_hidden, which was not given")
-            return self.suffix_forward(prefix_hidden)
+            return self.suffix_forward(prefix_hidden, targets, mask)
         if input_ids is None:
             raise ValueError(f"mode={mode!r} starts from input_ids, which were not given")
         hidden = self.prefix_forward(input_ids)
-        return hidden if mode == "prefix" else self.suffix_forward(hidden)
+        return hidden if mode == "prefix" else self.suffix_forward(hidden, targets, mask)
