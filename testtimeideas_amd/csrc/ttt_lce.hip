@@ -43,10 +43,8 @@ namespace {
 constexpr float kF16Scale = 16384.f;  // the largest stored magnitude: room below fp16's 65504 for rounding
 
 __host__ __device__ __forceinline__ int round8(int x) { return (x + 7) & ~7; }
-// Row stride of G and H of m columns: whole 128-byte lines, an odd number of
-// them.  With a power of two the 256 rows that a tile reads at once lie on a
-// few channels of the memory (8192 x 4096 x 32768 bf16 dX: 2281 us).
-__host__ __device__ __forceinline__ int piece_ld(int m) { return ((m + 63) / 64 | 1) * 64; }
+// Row stride of G and H of m columns: whole 128-byte lines of 16-bit values.
+__host__ __device__ __forceinline__ int piece_ld(int m) { return (m + 63) / 64 * 64; }
 
 // ---------------------------------------------------------------------------
 // Row copies of 16-bit operands: padded to 8 columns (zeros), and zeros in the
@@ -850,15 +848,17 @@ Buffers layout(const Plan& k, Carver* c) {
       b.nb = c->floats(k.V);
     }
   }
-  // parts: the most that any set of segments asks for
+  // parts: the most that any set of segments asks for; a product that is not
+  // split and not added to needs none
   int64_t px = 0, pw = 0;
+  const bool many = k.pieces > 1;
   for (int n = 1; n <= (gg ? 2 : 1); ++n) {
-    for (int keep = 0; keep < 2; ++keep) {
+    for (int keep = many; keep <= (many || gg); ++keep) {
       const int s = spread_x(k, n, keep).split;
-      if (s > px) px = s;
+      if ((keep || s > 1) && s > px) px = s;
     }
     const int s = spread_w(k, n).split;
-    if (s > pw) pw = s;
+    if (s > 1 && s > pw) pw = s;
   }
   b.part_x = c->floats(px * k.N * k.d);
   b.part_w = c->floats(pw * k.vc * k.d);
