@@ -108,10 +108,21 @@ def test_pieces_of_the_vocabulary(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
-def test_many_pieces_of_the_statistics(dtype):
-    """A vocabulary past one forward piece, few rows."""
-    s = _inputs(3, 16, 70001, dtype, seed=6)
+@pytest.mark.parametrize("vocab", [70001, 300001], ids=["one", "merged"])
+def test_large_vocabulary_of_few_rows(vocab, dtype):
+    """More vocabulary than a piece has, and more of its tiles' statistics than
+    are kept before they are merged."""
+    s = _inputs(3, 16, vocab, dtype, seed=6)
     _check(s, _run(s))
+
+
+@pytest.mark.parametrize("n", [1, 2, 5, 31, 32, 33, 63, 64, 65, 129])
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+def test_rows_of_the_joins(n, reduction):
+    """Each way in which a row's parts are read, and its last workgroup."""
+    s = _inputs(n, 40, 3000, torch.bfloat16, seed=60 + n, masked=n > 2)
+    up = torch.ones(n) if reduction == "none" else torch.tensor(1.0)
+    _check(s, _run(s, reduction=reduction, up=up), reduction=reduction, up=up.double())
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)

@@ -207,61 +207,93 @@ __global__ __launch_bounds__((kThreadsOf<T, SIZE>), 2) void k_logits(ZArgs a) {
     P::zero(u);
     tp.run(u, a.u, 0, list_steps<P::kStep>(a.u), lds);
   }
+  // Nothing from here on overlaps the products, so it is kept short: rows past
+  // M are made to count for nothing beforehand, where there are any, and the
+  // target, which few waves have, is put in afterwards.  In place of a test of
+  // both at every value (4096 x 1024 x 16384 bf16): forward 147 -> 132 us,
+  // backward 163 -> 146, double backward 344 -> 328.
+  if (tp.mrows < P::BM) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (tp.m_of(i) + e >= a.M)
+#pragma unroll
+          for (int j = 0; j < NI; ++j) z[i][j][e] = -__builtin_inff();
+  }
   const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
   for (int j = 0; j < NI; ++j) {
     const int n = tp.n_of(j);
     const bool nin = n < a.N;
     const int64_t td = nin ? a.target[n] - a.v0 : -1;  // the target's row in the piece
-    const int t = td >= 0 && td < a.M ? (int)td : -1;
+    // the target is value e of acc[i] for at = 16 i + e
+    const int at = td >= 0 && td < a.M ? (int)td - tp.m_of(0) : -1;
+    const bool hit = at >= 0 && at < 16 * MI && (at & 12) == 0;
+    const auto pick = [&](const auto& acc) {
+      float v = 0.f;
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v = at == 16 * i + e ? acc[i][j][e] : v;
+      return v;
+    };
+    const auto put = [&](auto& acc, float v) {
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = at == 16 * i + e ? v : acc[i][j][e];
+    };
     if constexpr (MODE == kStats) {
       float mx = -__builtin_inff();
 #pragma unroll
       for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int m = tp.m_of(i) + e;
-          if (m < a.M) mx = fmaxf(mx, z[i][j][e]);
-          if (m == t) a.at_target[n] = z[i][j][e];
-        }
+        for (int e = 0; e < 4; ++e) mx = fmaxf(mx, z[i][j][e]);
       mx = group_max(mx);
+      const float about = mx == -__builtin_inff() ? 0.f : mx;  // a wave whose rows are all past M: 0
       float s = 0.f;
 #pragma unroll
       for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          s += tp.m_of(i) + e < a.M ? fast_exp2((z[i][j][e] - mx) * kLog2e) : 0.f;
+        for (int e = 0; e < 4; ++e) s += fast_exp2((z[i][j][e] - about) * kLog2e);
       s = group_sum(s);
       if (g == 0 && nin) a.part[((int64_t)(tm * P::WM + tp.wm)) * a.N + n] = make_float2(mx, s);
+      if (hit) a.at_target[n] = pick(z);
     } else {
       const float mx = nin ? a.stat[n] : 0.f, inv = nin ? a.stat[a.N + n] : 0.f;
-      const float cm = MODE != kHSum && nin ? a.colmul[n] : 0.f;
-      const float h = MODE == kHGrad && nin ? a.h[n] : 0.f, q = MODE == kHGrad && nin ? a.q[n] : 0.f;
-      float hs = 0.f;
+      if constexpr (MODE == kHSum) {
+        float hs = 0.f;
 #pragma unroll
-      for (int i = 0; i < MI; ++i)
+        for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int m = tp.m_of(i) + e;
-          // rows of factor 0 are 0 whatever their logits are
-          const bool in = m < a.M && nin && (MODE == kHSum || cm != 0.f);
-          const float p = fast_exp2((z[i][j][e] - mx) * kLog2e) * inv;
-          if constexpr (MODE == kHSum) {
-            hs += in ? p * u[i][j][e] : 0.f;
-            if (m == t) a.at_target[n] = u[i][j][e];
-          } else {
-            // at the target from q: U there and h come from different sums, and p near 1 has their difference small
-            if constexpr (MODE == kHGrad) u[i][j][e] = in ? cm * p * (m == t ? -q : u[i][j][e] - h) : 0.f;
-            z[i][j][e] = in ? cm * (m == t ? p - 1.f : p) : 0.f;
-            if (sizeof(T) == 2 && m == t) {
-              if (a.rest_g) a.rest_g[n] = z[i][j][e] - (float)(T)z[i][j][e];
-              if (MODE == kHGrad && a.rest_h) a.rest_h[n] = u[i][j][e] - (float)(T)u[i][j][e];
-            }
+          for (int e = 0; e < 4; ++e) hs += fast_exp2((z[i][j][e] - mx) * kLog2e) * u[i][j][e];
+        hs = group_sum(hs) * inv;
+        if (g == 0 && nin) a.part[((int64_t)(tm * P::WM + tp.wm)) * a.N + n] = make_float2(hs, 0.f);
+        if (hit) a.at_target[n] = pick(u);
+      } else {
+        const float cm = nin ? a.colmul[n] : 0.f, h = MODE == kHGrad && nin ? a.h[n] : 0.f, ci = cm * inv;
+        const bool live = cm != 0.f;  // rows that do not count: 0 whatever their logits are
+        const float zt = hit ? pick(z) : 0.f;
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float cp = fast_exp2((z[i][j][e] - mx) * kLog2e) * ci;
+            if constexpr (MODE == kHGrad) u[i][j][e] = live ? cp * (u[i][j][e] - h) : 0.f;
+            z[i][j][e] = live ? cp : 0.f;
+          }
+        if (hit) {
+          const float p = fast_exp2((zt - mx) * kLog2e) * inv, gt = live ? cm * (p - 1.f) : 0.f;
+          put(z, gt);
+          if (sizeof(T) == 2 && a.rest_g) a.rest_g[n] = gt - (float)(T)gt;
+          if constexpr (MODE == kHGrad) {
+            // from q: U there and h come from different sums, and p near 1 has their difference small
+            const float ht = live ? -cm * p * a.q[n] : 0.f;
+            put(u, ht);
+            if (sizeof(T) == 2 && a.rest_h) a.rest_h[n] = ht - (float)(T)ht;
           }
         }
-      if constexpr (MODE == kHSum) {
-        hs = group_sum(hs);
-        if (g == 0 && nin) a.part[((int64_t)(tm * P::WM + tp.wm)) * a.N + n] = make_float2(hs, 0.f);
       }
     }
   }
@@ -424,6 +456,7 @@ struct RowArgs {
   const float* grad_loss;
   float* stat;  // [2N + 2]: max, 1/sum, 1/denominator, weight sum
   float* row;   // [N]: the rows' losses | the rows' shares of the upstream gradient's gradient
+  float2* sums;  // [ceil(N / 64)]: sums of losses and weights
   float* out;   // reduced
   float *h, *q;
   float *coef, *live, *colmul, *alpha;
@@ -442,26 +475,33 @@ __device__ __forceinline__ float2 join_stats(float2 a, float2 b) {
                              (b.y == 0.f ? 0.f : b.y * fast_exp2((b.x - mx) * kLog2e)));
 }
 
-// The parts' results of 64 tokens a workgroup, its sixteen waves taking a
-// part each in turn; to wave 0.
 template <bool STATS>
-__device__ __forceinline__ float2 join_parts(const float2* part, int parts, int N, int n, float2 (*lds)[64]) {
+__device__ __forceinline__ float2 join_two(float2 a, float2 b) {
+  if constexpr (STATS) return join_stats(a, b);
+  else return make_float2(a.x + b.x, 0.f);
+}
+
+// The parts' results of 64 tokens a workgroup, to the lanes of wave 0: lane l
+// has token *n (N: none).  All 1024 threads read parts, for fewer than 33
+// tokens too, where a wave takes several parts at once (1 token, 256 parts: 3.9
+// us in place of 5.5).
+template <bool STATS>
+__device__ __forceinline__ float2 join_parts(const float2* part, int parts, int N, int* n, float2 (*lds)[64]) {
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  int lanes = 64;
+  while (lanes / 2 >= N) lanes /= 2;  // lanes of a part
+  *n = blockIdx.x * 64 + lane % lanes;
   float2 s = make_float2(STATS ? -__builtin_inff() : 0.f, 0.f);
-  if (n < N)
+  if (*n < N)
 #pragma unroll 4
-    for (int i = w; i < parts; i += 16) {
-      const float2 p = part[(int64_t)i * N + n];
-      if constexpr (STATS) s = join_stats(s, p);
-      else s.x += p.x;
-    }
+    for (int i = (int)threadIdx.x / lanes; i < parts; i += 1024 / lanes)
+      s = join_two<STATS>(s, part[(int64_t)i * N + *n]);
+  for (int m = lanes; m < 64; m <<= 1) s = join_two<STATS>(s, make_float2(__shfl_xor(s.x, m), __shfl_xor(s.y, m)));
   lds[w][lane] = s;
   __syncthreads();
   if (w == 0)
-    for (int i = 1; i < 16; ++i) {
-      if constexpr (STATS) s = join_stats(s, lds[i][lane]);
-      else s.x += lds[i][lane].x;
-    }
+    for (int i = 1; i < 16; ++i) s = join_two<STATS>(s, lds[i][lane]);
+  if (lane >= lanes) *n = N;
   return s;
 }
 
@@ -484,8 +524,8 @@ __device__ __forceinline__ void finish_loss(const RowArgs& a, float l, float w) 
 // which keeps its digits where the target has nearly all of the probability.
 __global__ __launch_bounds__(1024) void k_join_loss(RowArgs a) {
   __shared__ float2 lds[16][64];
-  const int n = blockIdx.x * 64 + (threadIdx.x & 63);
-  const float2 s = join_parts<true>(a.part, a.parts, a.N, n, lds);
+  int n;
+  const float2 s = join_parts<true>(a.part, a.parts, a.N, &n, lds);
   if (threadIdx.x >= 64) return;
   float w = 0.f, wl = 0.f;
   if (n < a.N) {
@@ -496,15 +536,18 @@ __global__ __launch_bounds__(1024) void k_join_loss(RowArgs a) {
     wl = w == 0.f ? 0.f : w * l;
     a.row[n] = wl;
   }
-  // up to 64 rows: the whole reduction is here
-  if (gridDim.x == 1) finish_loss(a, wave_sum(wl), wave_sum(w));
+  wl = wave_sum(wl);
+  w = wave_sum(w);
+  // one workgroup (or nothing to reduce): the whole reduction is here
+  if (gridDim.x == 1 || (a.reduction == TTT_REDUCE_NONE && blockIdx.x == 0)) finish_loss(a, wl, w);
+  else if (threadIdx.x == 0) a.sums[blockIdx.x] = make_float2(wl, w);
 }
 
 // h = sum p U, and the rows' shares of the upstream gradient's gradient.
 __global__ __launch_bounds__(1024) void k_join_h(RowArgs a) {
   __shared__ float2 lds[16][64];
-  const int n = blockIdx.x * 64 + (threadIdx.x & 63);
-  const float2 s = join_parts<false>(a.part, a.parts, a.N, n, lds);
+  int n;
+  const float2 s = join_parts<false>(a.part, a.parts, a.N, &n, lds);
   if (threadIdx.x >= 64 || n >= a.N) return;
   a.h[n] = s.x;
   a.q[n] = s.x - a.at_target[n];
@@ -521,8 +564,8 @@ __global__ __launch_bounds__(1024) void k_join_h(RowArgs a) {
 template <bool STATS>
 __global__ __launch_bounds__(1024) void k_merge(float2* part, int parts, int N) {
   __shared__ float2 lds[16][64];
-  const int n = blockIdx.x * 64 + (threadIdx.x & 63);
-  const float2 s = join_parts<STATS>(part, parts, N, n, lds);
+  int n;
+  const float2 s = join_parts<STATS>(part, parts, N, &n, lds);
   if (threadIdx.x < 64 && n < N) part[n] = s;
 }
 
@@ -548,16 +591,14 @@ __device__ __forceinline__ float block_max(float v, float* lds) {
   return t;
 }
 
-// One workgroup: the rows' losses and weights to the loss and its denominator.
+// One workgroup: the sums of the workgroups of k_join_loss to the loss and its denominator.
 __global__ __launch_bounds__(1024) void k_reduce_loss(RowArgs a) {
   __shared__ float lds[16];
   float l = 0.f, w = 0.f;
-  if (a.reduction != TTT_REDUCE_NONE)
-#pragma unroll 4
-    for (int n = threadIdx.x; n < a.N; n += 1024) {
-      l += a.row[n];
-      w += row_weight(a, n);
-    }
+  for (int i = threadIdx.x; i < (a.N + 63) / 64; i += 1024) {
+    l += a.sums[i].x;
+    w += a.sums[i].y;
+  }
   l = block_sum(l, lds);
   w = block_sum(w, lds);
   finish_loss(a, l, w);
@@ -683,10 +724,10 @@ __global__ __launch_bounds__(256) void k_row_h(HArgs a) {
 // Host: sizes, workspace layout, launches.
 // ---------------------------------------------------------------------------
 constexpr int64_t kPieceBytes = 512ll << 20;  // G (and H) of a piece
-constexpr int64_t kPackBytes = 256ll << 20;   // copied head rows of a forward piece
+constexpr int64_t kPackBytes = 256ll << 20;   // copied head rows of a piece
+constexpr int64_t kPartBytes = 64ll << 20;    // the tiles' partial results that are kept before they are merged
+constexpr int kPieceRows = 131072;            // vocabulary rows of a piece at most
 constexpr int kMaxSplit = 64;
-constexpr int kMaxParts = 1024;    // rows of the tiles' partial results that are kept before they are merged
-constexpr int kStatsRows = 32768;  // vocabulary rows of a piece at most
 
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -695,36 +736,6 @@ struct Plan {
   bool f32, pack;  // pack: 16-bit rows are copied (not a multiple of 8 columns)
   int vc, pieces;  // vocabulary rows of a piece
 };
-
-Plan plan_of(const ttt_lce_problem* p, int entry) {
-  Plan k;
-  k.dtype = p->dtype;
-  k.entry = entry;
-  k.f32 = p->dtype == TTT_F32;
-  k.es = k.f32 ? 4 : 2;
-  k.N = (int)p->rows;
-  k.V = (int)p->vocab;
-  k.d = (int)p->cols;
-  k.dp = round8(k.d);
-  k.pack = !k.f32 && k.d % 8 != 0;
-  int64_t vc = kStatsRows;
-  if (entry == TTT_LCE_FWD) {
-    const int64_t fit = kPackBytes / ((int64_t)k.dp * 2);
-    if (k.pack && fit < vc) vc = fit;
-  } else {
-    vc = kPieceBytes / ((int64_t)k.N * k.es * (entry == TTT_LCE_BWD ? 1 : 2));
-  }
-  vc = vc / 256 * 256;
-  if (vc < 256) vc = 256;
-  if (vc > kStatsRows) vc = kStatsRows;
-  if (vc > p->vocab) vc = p->vocab;
-  k.pieces = (int)cdiv(p->vocab, vc);
-  vc = cdiv(cdiv(p->vocab, k.pieces), 256) * 256;
-  if (vc > p->vocab) vc = p->vocab;
-  k.vc = (int)vc;
-  k.pieces = (int)cdiv(p->vocab, vc);
-  return k;
-}
 
 // Hands out 256-byte aligned parts of the workspace; without one, counts.
 struct Carver {
@@ -764,6 +775,45 @@ int parts_of(const Plan& k, bool dual, int M, int N) {
   return (int)cdiv(M, tile_m(k, size)) * 2;
 }
 
+// Rows of parts that are kept before they are merged.
+int max_parts(const Plan& k) {
+  const int64_t n = kPartBytes / (8ll * k.N);
+  return (int)(n < 4 ? 4 : n > 16384 ? 16384 : n);
+}
+
+// The vocabulary's pieces.  As few as the bounds allow: a piece's tiles are
+// rounded up to whole rounds of the card (forward of 4096 x 1024 x 50001 bf16:
+// 13 rounds in one piece, 14 in two; 409 us, 1030 TFLOP/s).
+Plan plan_of(const ttt_lce_problem* p, int entry) {
+  Plan k;
+  k.dtype = p->dtype;
+  k.entry = entry;
+  k.f32 = p->dtype == TTT_F32;
+  k.es = k.f32 ? 4 : 2;
+  k.N = (int)p->rows;
+  k.V = (int)p->vocab;
+  k.d = (int)p->cols;
+  k.dp = round8(k.d);
+  k.pack = !k.f32 && k.d % 8 != 0;
+  int64_t vc = kPieceRows;
+  const auto bound = [&](int64_t rows) {
+    if (rows < vc) vc = rows;
+  };
+  if (k.pack) bound(kPackBytes / ((int64_t)k.dp * 2));
+  if (entry != TTT_LCE_FWD) bound(kPieceBytes / ((int64_t)k.N * k.es * (entry == TTT_LCE_BWD ? 1 : 2)));
+  if (entry != TTT_LCE_BWD)
+    while (vc > 256 && parts_of(k, entry == TTT_LCE_GG, (int)vc, k.N) > max_parts(k)) vc /= 2;
+  vc = vc / 256 * 256;
+  if (vc < 256) vc = 256;
+  if (vc > p->vocab) vc = p->vocab;
+  k.pieces = (int)cdiv(p->vocab, vc);
+  vc = cdiv(cdiv(p->vocab, k.pieces), 256) * 256;
+  if (vc > p->vocab) vc = p->vocab;
+  k.vc = (int)vc;
+  k.pieces = (int)cdiv(p->vocab, vc);
+  return k;
+}
+
 // The tile shape and split of a plain product of k in `segs` segments: the
 // least of (rounds of workgroups) x (steps of each) x (a step's time), plus the
 // parts' traffic where they are split.  Steps (us) at full occupancy, measured
@@ -801,7 +851,7 @@ struct Buffers {
   void *xr, *ar, *wr, *br;  // row copies
   void *g, *hh;
   float *part_x, *part_w;  // fp32 parts of dx, dw
-  float2* part;
+  float2 *part, *sums;
   float *at_target, *row, *h, *q, *coef, *live, *colmul, *rest_g, *rest_h, *alpha, *nx, *na, *nw, *nb;
   int parts;
 };
@@ -814,11 +864,12 @@ Buffers layout(const Plan& k, Carver* c) {
   if (fwd || gg) {
     const int whole = parts_of(k, gg, k.vc, k.N), last = parts_of(k, gg, k.V - (k.pieces - 1) * k.vc, k.N);
     const int64_t all = (int64_t)whole * (k.pieces - 1) + last;
-    b.parts = all <= kMaxParts ? (int)all : kMaxParts + (whole > last ? whole : last);
+    b.parts = all <= max_parts(k) ? (int)all : max_parts(k) + (whole > last ? whole : last);
   }
   if (b.parts) b.part = (float2*)c->take((int64_t)b.parts * k.N * 8);
   b.at_target = c->floats(k.N);
   b.row = c->floats(k.N);
+  if (fwd) b.sums = (float2*)c->take(cdiv(k.N, 64) * 8);
   if (!k.f32) {
     const int64_t xb = 2 * (int64_t)k.N * k.dp;
     if (k.pack || !fwd) b.xr = c->take(xb);
@@ -1019,6 +1070,7 @@ RowArgs row_args(const ttt_lce_problem* p, const Plan& k, const Buffers& b, cons
   r.grad_loss = grad_loss;
   r.part = b.part;
   r.at_target = b.at_target;
+  r.sums = b.sums;
   r.h = b.h;
   r.q = b.q;
   r.coef = b.coef;
@@ -1156,7 +1208,7 @@ int ttt_lce_fwd(const ttt_lce_problem* p, const ttt_rows* x, const ttt_rows* w, 
   r.row = p->reduction == TTT_REDUCE_NONE ? loss : b.row;
   r.out = loss;
   k_join_loss<<<(unsigned)cdiv(k.N, 64), 1024, 0, st>>>(r);
-  if (k.N > 64) k_reduce_loss<<<1, 1024, 0, st>>>(r);
+  if (k.N > 64 && p->reduction != TTT_REDUCE_NONE) k_reduce_loss<<<1, 1024, 0, st>>>(r);
   return finish("ttt_lce_fwd");
 }
 
