@@ -620,21 +620,33 @@ __global__ __launch_bounds__(1024) void k_factors(RowArgs a) {
     wm = block_max(wm, lds);
     bm = block_max(bm, lds);
   }
+  // kRows rows of a thread at a time: their loads, then the rest
+  constexpr int kRows = 4;
   const int stride = gridDim.x * 1024;
-#pragma unroll 4
-  for (int n = blockIdx.x * 1024 + threadIdx.x; n < a.N; n += stride) {
-    const float w = row_weight(a, n);
-    const float up = a.grad_loss[a.reduction == TTT_REDUCE_NONE ? n : 0];
-    const float c = w == 0.f ? 0.f : bad_target(a, n) ? __builtin_nanf("") : up * w * inv;
-    a.coef[n] = c;
-    a.live[n] = w == 0.f ? 0.f : 1.f;
-    if (a.dtype == TTT_F32) a.colmul[n] = c;
-    float t = fabsf(c);
-    if (a.nw || a.nb) {
-      const float ub = (a.na ? a.na[n] * wm : 0.f) + (a.nb ? a.nx[n] * bm : 0.f);
-      t *= fmaxf(1.f, 2.f * ub);
+  for (int n0 = blockIdx.x * 1024 + threadIdx.x; n0 < a.N; n0 += kRows * stride) {
+    int64_t t[kRows];
+    float w[kRows], up[kRows], ub[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const int n = n0 + i * stride;
+      const bool in = n < a.N;
+      t[i] = in ? a.target[n] : a.ignore;
+      w[i] = in && a.weight ? a.weight[n] : 1.f;
+      up[i] = in ? a.grad_loss[a.reduction == TTT_REDUCE_NONE ? n : 0] : 0.f;
+      ub[i] = (in && a.na ? a.na[n] * wm : 0.f) + (in && a.nx ? a.nx[n] * bm : 0.f);
     }
-    if (c != 0.f && t < __builtin_inff()) top = fmaxf(top, t);
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const int n = n0 + i * stride;
+      if (n >= a.N) break;
+      if (t[i] == a.ignore) w[i] = 0.f;
+      const float c = w[i] == 0.f ? 0.f : t[i] < 0 || t[i] >= a.V ? __builtin_nanf("") : up[i] * w[i] * inv;
+      a.coef[n] = c;
+      a.live[n] = w[i] == 0.f ? 0.f : 1.f;
+      if (a.dtype == TTT_F32) a.colmul[n] = c;
+      const float m = fabsf(c) * (a.nw || a.nb ? fmaxf(1.f, 2.f * ub[i]) : 1.f);
+      if (c != 0.f && m < __builtin_inff()) top = fmaxf(top, m);
+    }
   }
   if (a.dtype == TTT_F32) {
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.alpha = 1.f;
@@ -642,8 +654,14 @@ __global__ __launch_bounds__(1024) void k_factors(RowArgs a) {
   }
   top = fmaxf(block_max(top, lds), 1e-30f);
   const float s = (a.dtype == TTT_F16 ? kF16Scale : 1.f) / top;
-#pragma unroll 4
-  for (int n = threadIdx.x; n < a.N; n += 1024) a.colmul[n] = a.coef[n] * s;
+  for (int n0 = threadIdx.x; n0 < a.N; n0 += kRows * 1024) {  // this thread's rows of before
+    float c[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) c[i] = n0 + i * 1024 < a.N ? a.coef[n0 + i * 1024] : 0.f;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+      if (n0 + i * 1024 < a.N) a.colmul[n0 + i * 1024] = c[i] * s;
+  }
   if (threadIdx.x == 0) *a.alpha = a.dtype == TTT_F16 ? top * (1.f / kF16Scale) : top;
 }
 
@@ -655,18 +673,32 @@ __global__ __launch_bounds__(1024) void k_sum(const float* x, int n, float* out)
   if (threadIdx.x == 0) *out = s;
 }
 
-// norm[r] = |row r|, a wave a row.
+// norm[r] = |row r| of up to four operands in one launch, a wave a row.
+struct NormList {
+  struct {
+    const void* x;
+    int64_t ld;
+    int rows;
+    float* norm;
+  } s[4];
+  int n, cols;
+};
+
 template <typename T>
-__global__ __launch_bounds__(256) void k_norms(const T* x, int64_t ld, int R, int C, float* norm) {
-  const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (r >= R) return;
+__global__ __launch_bounds__(256) void k_norms(NormList a) {
+  int r = blockIdx.x * 4 + (threadIdx.x >> 6), i = 0;
+  const int lane = threadIdx.x & 63;
+  for (; i < a.n && r >= a.s[i].rows; ++i) r -= a.s[i].rows;
+  if (i >= a.n) return;
+  const T* x = (const T*)a.s[i].x + r * a.s[i].ld;
   float s = 0.f;
-  for (int c = lane; c < C; c += 64) {
-    const float v = (float)x[r * ld + c];
+#pragma unroll 4
+  for (int c = lane; c < a.cols; c += 64) {
+    const float v = (float)x[c];
     s += v * v;
   }
   s = wave_sum(s);
-  if (lane == 0) norm[r] = sqrtf(s);
+  if (lane == 0) a.s[i].norm[r] = sqrtf(s);
 }
 
 struct HArgs {
@@ -1278,10 +1310,14 @@ int ttt_lce_gg(const ttt_lce_problem* p, const ttt_rows* x, const ttt_rows* w, c
   const Call call{k, b, st};
   RowArgs r = row_args(p, k, b, target, row_weight, row_stats, grad_loss);
   if (k.dtype == TTT_F16) {
-    const auto norms = [&](const ttt_rows* t, int rows, float* out) {
-      k_norms<_Float16><<<(unsigned)cdiv(rows, 4), 256, 0, st>>>((const _Float16*)t->data, t->stride, rows, k.d, out);
+    NormList l{};
+    int64_t rows = 0;
+    const auto norms = [&](const ttt_rows* t, int n, float* out) {
+      l.s[l.n++] = {t->data, t->stride, n, out};
+      rows += n;
       return out;
     };
+    l.cols = k.d;
     if (has_a) {
       r.na = norms(ca, k.N, b.na);
       r.nw = norms(w, k.V, b.nw);
@@ -1290,6 +1326,7 @@ int ttt_lce_gg(const ttt_lce_problem* p, const ttt_rows* x, const ttt_rows* w, c
       r.nx = norms(x, k.N, b.nx);
       r.nb = norms(cb, k.V, b.nb);
     }
+    k_norms<_Float16><<<(unsigned)cdiv(rows, 4), 256, 0, st>>>(l);
   }
   launch_factors(r, st);
   const Operand xo = live_rows(k, x, b.xr, want_w, b.live, st);
