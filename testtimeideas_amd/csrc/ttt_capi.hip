@@ -632,7 +632,7 @@ void timing_mark(hipStream_t st, int tag, bool end) {
 
 extern "C" {
 
-int ttt_version(void) { return 500; }
+int ttt_version(void) { return 600; }
 
 int ttt_kernel_timing(int32_t capacity) {
   TimingPool& t = g_timing;
