@@ -323,3 +323,68 @@ def test_another_stream():
         got = _run(s)
     side.synchronize()
     assert all(torch.equal(got[k], ref[k]) for k in ref)
+
+
+def test_nan_stays_in_its_row():
+    s = _inputs(70, 64, 300, torch.bfloat16, seed=30)
+    bad = dict(s, x=s["x"].clone())
+    bad["x"][5, 3] = float("nan")
+    keep = torch.arange(70) != 5
+    for u in (True, False):
+        clean, got = (_run(t, reduction="none", up=torch.ones(70), names=("a",), up_grad=u) for t in (s, bad))
+        for k in ("rows", "dx", "gx"):
+            assert torch.equal(got[k][keep.cuda()], clean[k][keep.cuda()]), k
+            assert got[k][5].isnan().all(), k
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_one_tensor_as_both_operands(dtype):
+    """hidden and weight the same leaf: its gradients are the two operands' sums."""
+    s = _inputs(60, 48, 60, dtype, seed=31)
+    s["x"] = s["w"].clone()
+    apart = _run(s, up_grad=False)
+    t = s["w"].cuda().requires_grad_()
+    loss = linear_cross_entropy(t, t, s["t"].cuda())
+    dt, = torch.autograd.grad(loss, (t,), create_graph=True)
+    within("dt", dt, (apart["dx"].double() + apart["dw"].double()).cpu(),
+           torch.finfo(dtype).eps / 2 * (apart["dx"].double() + apart["dw"].double()).abs().cpu() + 1e-30)
+    # one cotangent serves both: gx and gw of a = b
+    s["b"] = s["a"]
+    apart = _run(s, up_grad=False)
+    gt, = torch.autograd.grad(dt, (t,), s["a"].cuda())
+    want = apart["gx"].double() + apart["gw"].double()
+    within("gt", gt, want.cpu(), torch.finfo(dtype).eps / 2 * want.abs().cpu() + 1e-30)
+
+
+def test_offsets_past_32_bits():
+    """A head of more than 2^31 values, zero but for its first and last rows:
+    against the formulas with the zero rows counted."""
+    n, d, v, k = 4, 4096, 600000, 3
+    g = torch.Generator().manual_seed(32)
+    ends = (torch.randn(2 * k, d, generator=g) * 2 / d ** 0.5).bfloat16()
+    x = torch.randn(n, d, generator=g).bfloat16()
+    rows = torch.tensor([0, 1, 2, v - 3, v - 2, v - 1, v // 2])  # the ends and one row of zeros
+    at = torch.tensor([4, 5, 0, 6])  # the targets' places among them
+    w = torch.zeros(v, d, dtype=torch.bfloat16, device="cuda")
+    w[:k], w[-k:] = ends[:k].cuda(), ends[k:].cuda()
+    w.requires_grad_()
+    xd = x.cuda().requires_grad_()
+    loss = linear_cross_entropy(xd, w, rows[at].cuda())
+    dx, dw = torch.autograd.grad(loss, (xd, w))
+
+    x, we = x.double(), torch.cat([ends.double(), torch.zeros(1, d).double()])
+    z = x @ we.T
+    lse = torch.log(z[:, :-1].exp().sum(1) + (v - 2 * k))
+    grad = (z - lse[:, None]).exp()
+    grad[torch.arange(n), at] -= 1
+    grad /= n
+    # products of d terms in fp32 make z, whose error is p's relative one; G and the results are rounded to bf16
+    ez = d * 2.0 ** -24 * (x.abs() @ we.abs().T).max().item()
+    unit = 2.0 ** -8
+    within("loss", loss, (lse - z[torch.arange(n), at]).mean(), torch.tensor(2 * ez + 1e-5))
+    within("dx", dx, grad @ we, (2 * unit + 2 * ez) * (grad.abs() @ we.abs()) + 1e-30)
+    within("dw", dw[rows.cuda()], grad.T @ x, (2 * unit + 2 * ez) * (grad.abs().T @ x.abs()) + 1e-30)
+    # the zero rows in between all have the same gradient
+    other = (-lse).exp() / n
+    for j in (k, 524288, 599000):
+        within(f"dw[{j}]", dw[j], other @ x, (2 * unit + 2 * ez) * (other.abs() @ x.abs()) + 1e-30)

@@ -233,3 +233,18 @@ def test_another_stream():
         got = _run(s)
     side.synchronize()
     assert all(torch.equal(got[k], ref[k]) for k in ref)
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 values: the last rows against the formulas."""
+    n, d = 66000, 32768
+    s = _inputs(3, d, torch.bfloat16, seed=21)
+    x = torch.zeros(n, d, dtype=torch.bfloat16, device="cuda")
+    dy = torch.zeros_like(x)
+    x[-3:], dy[-3:] = s["x"].cuda(), s["dy"].cuda()
+    x.requires_grad_()
+    y = layer_norm(x, s["w"].cuda(), s["b"].cuda(), EPS)
+    dx, = torch.autograd.grad(y, (x,), dy)
+    _check(s, {"y": y[-3:], "dx": dx[-3:]})
+    # a row of zeros: the bias, and no gradient
+    assert torch.equal(y[0].cpu(), s["b"]) and not dx[:-3].any()
