@@ -388,3 +388,22 @@ def test_offsets_past_32_bits():
     other = (-lse).exp() / n
     for j in (k, 524288, 599000):
         within(f"dw[{j}]", dw[j], other @ x, (2 * unit + 2 * ez) * (other.abs() @ x.abs()) + 1e-30)
+
+
+def test_fp32_errors_have_no_common_sign():
+    """Sums over many rows would gather one.  The rows' errors are independent,
+    so their mean is within four deviations, 4 / sqrt(rows) of their root mean
+    square."""
+    n = 8000
+    s = _inputs(n, 100, 1700, torch.float32, seed=40)
+    got = _run(s, names=("a",), up_grad=False)
+    d = {k: s[k].double().cuda() for k in ("x", "w", "a")}
+    p = torch.softmax(d["x"] @ d["w"].T, 1)
+    u = d["a"] @ d["w"].T
+    h = p * (u - (p * u).sum(1, keepdim=True))
+    g = p.clone()
+    g[torch.arange(n), s["t"].cuda()] -= 1
+    ref = dict(dx=g @ d["w"] / n, gx=h @ d["w"] / n)
+    for k, want in ref.items():
+        err = got[k].double() - want
+        assert err.mean().abs() < 4 / n ** 0.5 * err.square().mean().sqrt(), k
