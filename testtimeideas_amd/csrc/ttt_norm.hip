@@ -147,9 +147,9 @@ __device__ __forceinline__ void load_row(const void* x, int64_t ld, int64_t row,
 // WHOLE: rows are whole chunks.  The loads of a part of a chunk, value by value,
 // take up to 32 registers, and rows in flight with them (8192 x 2048 bf16: gg
 // 50 -> 39 us; forward, with the parameters loaded once, 27 -> 14 us).  Measured:
-// 65536 x 4096 bf16 forward 211 us, backward 300 us, both at the 5.0 to 5.4 TB/s
-// of a large copy; 8192 x 384 fp32 forward 9.3, backward 9.9, gg 16.2 us (a copy
-// of as many bytes: 5, 8 and 13).
+// 65536 x 4096 bf16 forward 208 us, backward 296 us, both at the 5.0 to 5.4 TB/s
+// of a large copy; 8192 x 384 fp32 forward 9.4, backward 11.1, gg 18.1 us (a
+// copy of as many bytes: 5, 8 and 13).
 //
 // Every kernel walks its rows with the next row's loads in flight while this
 // row is reduced and stored.  Rows past 2^31 - 1 do not exist, but row + stride
