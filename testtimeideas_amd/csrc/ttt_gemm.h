@@ -694,7 +694,8 @@ struct DirectProduct : TileBase<32, 32, 2, 2, 32> {
 // Tile (tm, tn) of workgroup `id` among tm_count x tn_count.  Workgroups go to
 // the eight XCDs in turn, each with an L2 of its own: an XCD gets a run of
 // neighbouring tiles, walked in blocks of kGroup tn, so that the tiles in
-// flight on it share operand rows.
+// flight on it share operand rows.  (kGroup 4, 2, 8: 8192 x 4096 x 65536 bf16
+// forward 3290, 3313, 3316 us; 4096 x 1024 x 16384 134, 135, 131.)
 __device__ __forceinline__ void tile_of(int id, int tm_count, int tn_count, int* tm, int* tn) {
   constexpr int kXcd = 8, kGroup = 4;
   const int total = tm_count * tn_count;
